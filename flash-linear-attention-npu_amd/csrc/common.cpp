@@ -27,7 +27,7 @@ int check_tensor(const fla_tensor *t, const char *op, const char *name, int ndim
     if (ndim >= 0 && t->ndim != ndim)
         return fail(FLA_ERR_SHAPE, "%s: %s must be rank %d, got rank %d.", op, name, ndim, t->ndim);
     if (t->ndim < 0 || t->ndim > FLA_MAX_DIMS) return fail(FLA_ERR_SHAPE, "%s: %s has invalid rank.", op, name);
-    if (t->dtype < 0 || t->dtype > FLA_I64 || !(dtype_mask & dt_bit(t->dtype)))
+    if (t->dtype < 0 || t->dtype > FLA_F8E4M3 || !(dtype_mask & dt_bit(t->dtype)))
         return fail(FLA_ERR_DTYPE, "%s: %s has unsupported dtype %d.", op, name, t->dtype);
     for (int i = 0; i < t->ndim; ++i)
         if (t->shape[i] < 0) return fail(FLA_ERR_SHAPE, "%s: %s has a negative extent.", op, name);

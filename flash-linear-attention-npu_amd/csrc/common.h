@@ -52,6 +52,7 @@ inline size_t dtype_size(int dt) {
         case FLA_F32: case FLA_I32: return 4;
         case FLA_F16: case FLA_BF16: return 2;
         case FLA_I64: return 8;
+        case FLA_I8: case FLA_F8E4M3: return 1;
         default: return 0;
     }
 }

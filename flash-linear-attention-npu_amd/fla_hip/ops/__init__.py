@@ -13,7 +13,9 @@ import functools
 import inspect
 from typing import Callable
 
+from . import _paged_kv
 from ._hip_ctypes import HIP_CTYPES_OPS, chunk_kda_fwd_noalloc, gdn_chunk_fwd, l2norm_bwd, l2norm_fwd
+from ._paged_kv import rotary_axes_bwd, rotary_axes_fwd
 
 _REFERENCE_OPS = (
     "npu_fast_gelu_custom",
@@ -48,10 +50,14 @@ MUTATED_ARGUMENTS = {
     "npu_recurrent_kda": ("initial_state",),
     "recurrent_gated_delta_rule": ("state",),
     "npu_recurrent_gated_delta_rule": ("state",),
+    "paged_kv_plan": ("block_table",),
+    "paged_kv_append": ("key_cache", "value_cache", "key_scales", "value_scales"),
+    "paged_kv_attention": ("out",),
 }
 
 MUTATION_PREDICATES = {
     "npu_recurrent_kda": lambda arguments: bool(arguments["inplace_final_state"]),
+    "paged_kv_attention": lambda arguments: arguments["out"] is not None,
 }
 
 
@@ -84,7 +90,8 @@ def _wrap_mutable_op(name: str, op: Callable) -> Callable:
                 "must not require gradients; use a functional state API for training."
             )
         result = op(*args, **kwargs)
-        touched = [value for value in targets.values() if isinstance(value, torch.Tensor)]
+        # tensors made in inference mode have no version counter
+        touched = [value for value in targets.values() if isinstance(value, torch.Tensor) and not value.is_inference()]
         if touched:
             torch.autograd.graph.increment_version(touched)
         return result
@@ -108,6 +115,10 @@ for _name in _REFERENCE_OPS:
     _op = _missing_op(_name) if _op is None else _wrap_mutable_op(_name, _op)
     globals()[_name] = _op
     globals()[_strip_npu_prefix(_name)] = _op
+
+
+for _name in ("paged_kv_plan", "paged_kv_append", "paged_kv_attention"):
+    globals()[_name] = _wrap_mutable_op(_name, getattr(_paged_kv, _name))
 
 
 def _has_tensor_requiring_grad(*tensors) -> bool:
@@ -162,6 +173,39 @@ def causal_conv1d(x, weight, bias=None, conv_states=None, *, query_start_loc=Non
     return Function.apply(x, weight, bias, conv_states)
 
 
+def rotary_axes(q, k, positions, inv_freq, sections, *, axis_order="blocked", pairing="half"):
+    """Rotary positions with one or more axes (text; height and width; time, height and width), differentiable in q and k.
+
+    ``q``, ``k`` (or None) ``[B, T, H, D]`` or ``[T, H, D]`` in bf16, fp16 or fp32, with any outer strides and numbers of heads of
+    their own; ``positions`` int32 or int64 ``[axes, B, T]`` or ``[axes, T]``; ``inv_freq`` fp32 ``[R / 2]`` on the device;
+    ``sections``: frequencies of each axis, summing to R / 2, given out in contiguous blocks (``axis_order="blocked"``) or to the
+    axes in turn while they have any left (``"interleaved"``).  Channel pair j turns by ``positions[axis_j] * inv_freq[j]``
+    (formed in 64 bits); a pair is channels j and j + R/2 (``pairing="half"``) or 2j and 2j + 1 (``"adjacent"``).  Channels
+    from R on pass through.  Returns the rotated q and k in the memory order of the inputs."""
+    import torch
+
+    how = dict(axis_order=axis_order, pairing=pairing)
+    if not _has_tensor_requiring_grad(q, k):
+        return rotary_axes_fwd(q, k, positions, inv_freq, sections, **how)
+
+    class Function(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q_, k_):
+            ctx.save_for_backward(positions, inv_freq)
+            return rotary_axes_fwd(q_, k_, positions, inv_freq, sections, **how)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, dq, dk):
+            turned = ctx.saved_tensors
+            grads = [None if g is None else g if g.stride(-1) == 1 else g.contiguous() for g in (dq, dk)]
+            if grads[0] is None:
+                return None, rotary_axes_bwd(grads[1], None, *turned, sections, **how)[0]
+            return rotary_axes_bwd(*grads, *turned, sections, **how)
+
+    return Function.apply(q, k)
+
+
 __all__ = [
     "MUTATED_ARGUMENTS",
     "MUTATION_PREDICATES",
@@ -169,6 +213,12 @@ __all__ = [
     "gdn_chunk_fwd",
     "l2norm_bwd",
     "l2norm_fwd",
+    "paged_kv_append",
+    "paged_kv_attention",
+    "paged_kv_plan",
+    "rotary_axes",
+    "rotary_axes_bwd",
+    "rotary_axes_fwd",
     *sorted(set(_REFERENCE_OPS)),
     *sorted({_strip_npu_prefix(n) for n in _REFERENCE_OPS}),
 ]

@@ -7,6 +7,7 @@ call :388-429, entry ``call_aclnn`` :463-482).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Callable, Iterable, Optional, Sequence
 
@@ -201,6 +202,27 @@ def call_op(name: str, argtypes: Sequence, build_args: Callable[[CallContext], l
     return outputs
 
 
+def bind_direct(name: str, argtypes: Sequence):
+    """``fla_<name>`` as a one-phase entry point (no workspace) with explicit argtypes."""
+    launch = _BOUND.get(name)
+    if launch is None:
+        launch = getattr(_library(), f"fla_{name}")
+        launch.argtypes = [*argtypes, ctypes.c_void_p]
+        launch.restype = ctypes.c_int
+        _BOUND[name] = launch
+    return launch
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_guard(device):
+    """Makes ``device`` current for the time of a call; nothing to do where it is already."""
+    import torch
+
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def call_op_noalloc(name: str, argtypes: Sequence, build_args: Callable[[CallContext], list], outputs):
     """One-phase call of ``fla_<name>(<operands>, stream)``: an entry point that brings its own scratch memory.
     Nothing is allocated here or inside the library; the caller has allocated ``outputs``."""
@@ -211,12 +233,7 @@ def call_op_noalloc(name: str, argtypes: Sequence, build_args: Callable[[CallCon
         raise RuntimeError(f"fla_{name}: no output tensor to take the device from.")
     ensure_gpu_tensor(anchor, "output")
     device = anchor.device
-    launch = _BOUND.get(name)
-    if launch is None:
-        launch = getattr(_library(), f"fla_{name}")
-        launch.argtypes = [*argtypes, ctypes.c_void_p]
-        launch.restype = ctypes.c_int
-        _BOUND[name] = launch
+    launch = bind_direct(name, argtypes)
     with torch.cuda.device(device):
         ctx = CallContext(device)
         args = build_args(ctx)

@@ -44,7 +44,9 @@ typedef enum fla_dtype {
     FLA_F16 = 1,
     FLA_BF16 = 2,
     FLA_I32 = 3,
-    FLA_I64 = 4
+    FLA_I64 = 4,
+    FLA_I8 = 5,
+    FLA_F8E4M3 = 6           /* OCP e4m3: no infinities, largest value 448      */
 } fla_dtype;
 
 typedef enum fla_status {
@@ -773,6 +775,74 @@ int fla_prepare_wy_repr_bwd_full_accumulate(
     const fla_int_array *chunk_indices, int64_t chunk_size, const fla_tensor *k_rstd, const fla_tensor *dk,
     const fla_tensor *dv, const fla_tensor *dbeta, const fla_tensor *dg, void *workspace, uint64_t workspace_size,
     void *stream);
+
+/* ------------------------------------------------------------------------
+ * Softmax attention over a paged cache held in 8 bits, with the plan of its pages, the positions of its queries and
+ * keys and the append that fills it: the layers that stand between linear-attention layers in a hybrid stack.  No
+ * counterpart in the reference.  The cache is a pool of pages of `block_size` tokens (a power of two, 16 .. 256):
+ * codes [P,H,block_size,D] of type FLA_F8E4M3 or FLA_I8 and one fp32 scale for each page and head, [P,H]; a stored
+ * value is code * scale.  All lengths, tables and slots are read on the device, so every call may be captured into a
+ * graph and replayed with other contents.
+ *
+ * paged_kv_plan: where the tokens of this step go.  context_lens, query_lens i32 [N]: tokens a request has in the
+ * cache, and tokens it adds.  block_table i32 [N,M] (unit innermost stride): the pages of each request in order; the
+ * entries of the pages that this step opens, ceil(context/block) <= j < ceil((context + query)/block), j < M, are
+ * written, request by request, from free_blocks i32 [F] front to back, or -1 once the list has run out.  Written:
+ * slot_mapping i64 [T] (page * block_size + offset in the page of each new token in request order; -1 where a token
+ * has no page and behind the last token), positions i32 [T] (0 behind the last token), cu_seqlens i32 [N+1],
+ * seq_lens i32 [N] (context + query), blocks_used i32 [1] (entries of free_blocks that the step needs: more than F
+ * means that the list ran out), and with state_rows i32 [N] state_indices i32 [T] (the request's row for each token,
+ * as recurrent_gated_delta_rule takes them; -1 behind the last token; NULL with state_rows NULL).  Negative lengths
+ * count as 0.  T may be larger than the number of new tokens (padding) or smaller (later tokens are dropped).
+ * ------------------------------------------------------------------------ */
+int fla_paged_kv_plan(
+    const fla_tensor *context_lens, const fla_tensor *query_lens, const fla_tensor *block_table,
+    const fla_tensor *free_blocks, const fla_tensor *state_rows, int64_t block_size,
+    const fla_tensor *slot_mapping, const fla_tensor *positions, const fla_tensor *cu_seqlens,
+    const fla_tensor *seq_lens, const fla_tensor *blocks_used, const fla_tensor *state_indices, void *stream);
+
+/* rotary_axes: rotary positions with one or more axes (text; height and width; time, height and width).  x [B,T,H,D]
+ * or [T,H,D], bf16, f16 or f32, unit innermost stride, free outer strides: q and optionally k (NULL), rotated into q_out
+ * and k_out of the same shapes; positions i32 or i64 [A,B,T] or [A,T]; inv_freq f32 [R/2] (device); axis_of_freq: host
+ * array of R/2 axes (0 .. A-1).  Channel pair j turns by positions[axis_of_freq[j]] * inv_freq[j] (formed in 64 bits):
+ * (a, b) -> (a cos - b sin, b cos + a sin), the pair being channels j and j + R/2, or 2j and 2j + 1 with adjacent.
+ * Channels from R on are copied.  inverse: turns by the negative angle, which is the gradient of the operator. */
+int fla_rotary_axes(
+    const fla_tensor *q, const fla_tensor *k, const fla_tensor *positions, const fla_tensor *inv_freq,
+    const fla_int_array *axis_of_freq, bool adjacent, bool inverse, const fla_tensor *q_out,
+    const fla_tensor *k_out, void *stream);
+
+/* paged_kv_append: quantises the rows of key and value ([T,H,D] bf16, f16 or f32) into the pages that slot_mapping
+ * i64 [T] names (negative or past the pool: the row is skipped).  The rows of one page must follow each other with
+ * ascending slots, as paged_kv_plan lays them out; a page named by two separate runs of rows in one call has
+ * unspecified contents.  Page tokens before the first new one are kept, those behind the last new one are left alone.
+ * A page's scale is the smallest power of two s (at least 2^-126) with max|x| / s <= 448 (e4m3) or 127 (int8) over the
+ * finite elements stored so far in that page and head, 0 while all are 0; when it grows, the codes already there are
+ * converted to it.  Codes are x / s rounded to nearest even; infinities store the largest code, NaN stores NaN (e4m3)
+ * or 0 (int8). */
+int fla_paged_kv_append(
+    const fla_tensor *key, const fla_tensor *value, const fla_tensor *key_cache, const fla_tensor *value_cache,
+    const fla_tensor *key_scales, const fla_tensor *value_scales, const fla_tensor *slot_mapping, void *stream);
+
+/* paged_kv_attention: out = softmax(scale * q k^T) v over the cached tokens of each request.  query, out [T,Hq,D] bf16
+ * or f16 (D = 64, 128 or 256; Hq a multiple of the cache's heads); seq_lens i32 [N]: tokens in the cache, the new ones
+ * included; cu_seqlens i32 [N+1]: the query rows of each request (NULL: one row for each request, T = N).  Query row j
+ * of the q rows of request r is token seq_lens[r] - q + j and sees the tokens up to itself.  Pages that block_table
+ * ([N,M] i32) gives a number outside the pool are not seen.  A row that sees nothing is 0 with lse -inf.  lse f32 [T,Hq]
+ * optional: natural logarithm of the sum of exponentials.  max_query_len: the largest number of query rows of a request
+ * (a hint that chooses the kernel; 0: unknown).  Rows behind the last request are left as they are, or set to 0 (lse
+ * -inf) with clear_tail.  Codes behind a request's last token are never read into a result. */
+int fla_paged_kv_attention_get_workspace_size(
+    const fla_tensor *query, const fla_tensor *key_cache, const fla_tensor *value_cache,
+    const fla_tensor *key_scales, const fla_tensor *value_scales, const fla_tensor *block_table,
+    const fla_tensor *seq_lens, const fla_tensor *cu_seqlens, double scale, int64_t max_query_len,
+    bool clear_tail, const fla_tensor *out, const fla_tensor *lse, uint64_t *workspace_size);
+int fla_paged_kv_attention(
+    const fla_tensor *query, const fla_tensor *key_cache, const fla_tensor *value_cache,
+    const fla_tensor *key_scales, const fla_tensor *value_scales, const fla_tensor *block_table,
+    const fla_tensor *seq_lens, const fla_tensor *cu_seqlens, double scale, int64_t max_query_len,
+    bool clear_tail, const fla_tensor *out, const fla_tensor *lse, void *workspace,
+    uint64_t workspace_size, void *stream);
 
 #ifdef __cplusplus
 }

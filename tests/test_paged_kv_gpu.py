@@ -1,0 +1,596 @@
+"""Paged 8-bit cache operators against their 64-bit restatement.
+
+Bounds (eps = torch.finfo(type).eps; a rounding is off by at most eps / 2 of the value):
+* plan, append: equal.  Scales are powers of two, so x / scale is exact and the code is one rounding of it.
+* rotary: one rounding to the output type, plus fp32 arithmetic on (a, b): the sine and cosine are within 2^-22 (an fp32
+  fraction of a turn, 2^-24 of at most pi, and the function's own 2^-23), two products and a sum add 3 * 2^-24 of
+  |a| + |b| <= 2^-21 (|a| + |b|) in all.
+* attention: one rounding to the output type.  Every weight carries 2^-12 (fp16) and the error of its score: a sum of D
+  products in fp32, at most (D + 8) * 2^-24 of sum |q||k| * scale, twice (weight and normalisation).  These are relative
+  errors of weights, so they count for sum p|v| ("spread").  A weight below 2^-14 is off by at most 2^-25 of
+  the largest scale times the largest code, for each token.  lse: the score error, and 2^-21 of its value.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+from oracle import paged_kv as ref
+
+pytestmark = pytest.mark.gpu
+E4M3, INT8 = torch.float8_e4m3fn, torch.int8
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+# ---- plan ------------------------------------------------------------------------------------------------------------
+
+def make_plan(n, page, seed, most_context, most_query, spare=3, width_cut=0):
+    rng = random.Random(seed)
+    context = [rng.choice([0, 1, page - 1, page, page + 1, rng.randint(0, most_context)]) for _ in range(n)]
+    query = [rng.choice([0, 1, 1, rng.randint(0, most_query)]) for _ in range(n)]
+    width = max(1, max(-(-(c + q) // page) for c, q in zip(context, query)) - width_cut)
+    ids = list(range(100000))
+    rng.shuffle(ids)
+    table = []
+    for c in context:
+        held = min(-(-c // page), width)
+        table.append([ids.pop() for _ in range(held)] + [-7] * (width - held))
+    need = sum(min(-(-(c + q) // page), width) - min(-(-c // page), width) for c, q in zip(context, query))
+    free = [ids.pop() for _ in range(max(0, need + spare))]
+    return context, query, table, free
+
+
+@pytest.mark.parametrize("n,page,most_context,most_query,pad,spare,cut", [
+    (1, 16, 40, 1, 0, 3, 0), (3, 64, 300, 5, 4, 0, 0), (7, 32, 0, 200, 0, 1, 0), (257, 16, 90, 3, 31, 9, 0),
+    (1030, 16, 40, 4, 0, 0, 0), (2500, 64, 100, 3, 1000, 2, 0), (5, 256, 1000, 3000, 7, 0, 0),
+    (9, 16, 200, 60, -50, 0, 0), (40, 16, 100, 40, 3, -5, 0), (12, 32, 300, 100, 0, 2, 2)])
+def test_plan(dev, n, page, most_context, most_query, pad, spare, cut):
+    from fla_hip import ops
+    context, query, table, free = make_plan(n, page, 7 * n + page, most_context, most_query, spare, cut)
+    tokens = max(0, sum(query) + pad)
+    rows = random.Random(n).sample(range(5000), n)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    wide = torch.full((n, len(table[0]) + 3), -9, dtype=torch.int32, device=dev)     # rows that are not adjacent
+    wide[:, :-3] = i32(table)
+    view = wide[:, :-3]
+    got = ops.paged_kv_plan(i32(context), i32(query), view, i32(free), page, tokens, state_rows=i32(rows))
+    want = ref.plan(context, query, table, free, page, tokens, rows)
+    for name, g in zip(("slots", "positions", "cu", "seq", "used", "states"), got):
+        assert g.dtype == want[name].dtype and torch.equal(g.cpu(), want[name]), name
+    assert torch.equal(view.cpu(), want["table"])
+    assert bool((wide[:, -3:] == -9).all())
+    assert ops.paged_kv_plan(i32(context), i32(query), view, i32(free), page, tokens)[5] is None
+
+
+def test_plan_negative_lengths_count_as_zero_and_nothing_to_do(dev):
+    from fla_hip import ops
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    table = torch.full((3, 2), -1, dtype=torch.int32, device=dev)
+    slots, pos, cu, seq, used, _ = ops.paged_kv_plan(i32([-4, 3, 0]), i32([2, -1, 0]), table, i32([5]), 16, 3)
+    assert slots.tolist() == [80, 81, -1] and cu.tolist() == [0, 2, 2, 2] and seq.tolist() == [2, 3, 0] and used.tolist() == [1]
+    assert table.tolist() == [[5, -1], [-1, -1], [-1, -1]]
+    empty = torch.empty(0, dtype=torch.int32, device=dev)
+    slots, pos, cu, seq, used, _ = ops.paged_kv_plan(i32([4]), i32([0]), table[:1], empty, 16, 0)
+    assert slots.numel() == 0 and cu.tolist() == [0, 0] and used.tolist() == [0]
+    slots, pos, cu, seq, used, st = ops.paged_kv_plan(empty, empty, table[:0], empty, 16, 2, state_rows=empty)
+    assert slots.tolist() == [-1, -1] and cu.tolist() == [0] and st.tolist() == [-1, -1] and used.tolist() == [0]
+
+
+# ---- rotary ----------------------------------------------------------------------------------------------------------
+
+def rotary_bound(x, want, rotated, pairing, dtype):
+    """Elementwise bound of the module's docstring."""
+    half = rotated // 2
+    a = x.double().abs()
+    first, second = (slice(0, rotated, 2), slice(1, rotated, 2)) if pairing == "adjacent" else (slice(0, half), slice(half, rotated))
+    pair = torch.zeros_like(a)
+    pair[..., first] = pair[..., second] = a[..., first] + a[..., second]
+    return want.abs() * torch.finfo(dtype).eps / 2 * 1.01 + pair * 2.0 ** -21 + torch.finfo(dtype).tiny
+
+
+ROTARY = [
+    # batch, tokens, q heads, k heads, dim, rotated, sections, order, pairing, dtype
+    ((), 1, 4, 1, 128, 128, (64,), "blocked", "half", BF),
+    ((), 33, 5, 2, 64, 64, (12, 10, 10), "interleaved", "half", F16),
+    ((2,), 65, 32, 8, 128, 64, (16, 8, 8), "blocked", "half", BF),
+    ((2,), 9, 3, 3, 256, 64, (11, 11, 10), "interleaved", "adjacent", BF),
+    ((), 4100, 2, 1, 64, 32, (8, 8), "blocked", "adjacent", F32),
+    ((), 17, 3, 0, 80, 40, (20,), "blocked", "half", BF),            # pieces of 4
+    ((3,), 5, 2, 1, 34, 18, (4, 3, 2), "interleaved", "half", F16),   # single elements
+    ((), 7, 2, 1, 6, 6, (3,), "blocked", "adjacent", F32),
+    ((), 21, 2, 2, 256, 256, (64, 32, 32), "blocked", "half", F32),
+]
+
+
+@pytest.mark.parametrize("batch,T,hq,hk,dim,rotated,sections,order,pairing,dtype", ROTARY)
+@pytest.mark.parametrize("head_first", [False, True])
+def test_rotary_forward_and_gradient(dev, batch, T, hq, hk, dim, rotated, sections, order, pairing, dtype, head_first):
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(T * dim)
+
+    def new(h):
+        x = torch.randn(*batch, T, h, dim, generator=gen).to(dtype).to(dev)
+        return x.transpose(-2, -3).contiguous().transpose(-2, -3) if head_first else x
+
+    q, k = new(hq), new(hk) if hk else None
+    pos = torch.randint(0, 1 << 20, (len(sections), *batch, T), generator=gen)
+    pos.flatten()[0] = 1 << 30
+    inv = (10000.0 ** (-torch.arange(rotated // 2, dtype=torch.float64) / (rotated // 2))).float()
+    args = (pos.to(dev) if T % 2 else pos.int().to(dev), inv.to(dev), sections)
+    how = dict(axis_order=order, pairing=pairing)
+    xs = [x for x in (q, k) if x is not None]
+    for x in xs:
+        x.requires_grad_()
+    got = ops.rotary_axes(q, k, *args, **how)
+    grads = [torch.randn(x.shape, generator=gen).to(dtype).to(dev) for x in xs]
+    back = torch.autograd.grad([g for g in got if g is not None], xs, grads)
+    assert (got[1] is None) == (k is None)
+    for x, y, dy, dx in zip(xs, got, grads, back):
+        assert y.dtype == dtype and y.stride() == x.stride()
+        for source, result, inverse in ((x, y, False), (dy, dx, True)):
+            want = ref.rotary(source.detach().cpu(), pos, inv, sections, order, pairing, inverse)
+            error = (result.detach().cpu().double() - want).abs()
+            bound = rotary_bound(source.detach().cpu(), want, rotated, pairing, dtype)
+            assert bool((error <= bound).all()), float((error / bound).max())
+        assert torch.equal(y[..., rotated:], x.detach()[..., rotated:])
+
+
+def test_rotary_gradient_against_differences(dev):
+    """The operator is linear in x: central differences in fp32 with a step of 1 are exact up to rounding (2^-21 of the pair,
+    twice, each way)."""
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(3, 2, 16, generator=gen).to(dev).requires_grad_()
+    pos, inv, dy = torch.randint(0, 999, (2, 3), generator=gen).to(dev), torch.rand(4, generator=gen).to(dev), torch.randn(3, 2, 16, generator=gen).to(dev)
+    y, _ = ops.rotary_axes(x, None, pos, inv, (2, 2), pairing="adjacent")
+    (dx,) = torch.autograd.grad(y, x, dy)
+    with torch.no_grad():
+        for i in (0, 1, 6, 7, 8, 15):
+            step = torch.zeros_like(x)
+            step[1, 1, i] = 1
+            plus, minus = (ops.rotary_axes(x + s * step, None, pos, inv, (2, 2), pairing="adjacent")[0] for s in (1, -1))
+            num = ((plus - minus).double() * dy.double()).sum() / 2
+            assert abs(float(num) - float(dx[1, 1, i])) <= 16 * 2.0 ** -21 * float(dy[1, 1].abs().sum()), i
+
+
+def test_rotary_one_gradient_only_and_expanded_gradient(dev):
+    from fla_hip import ops
+    q, k = torch.randn(5, 2, 64, device=dev, requires_grad=True), torch.randn(5, 1, 64, device=dev, requires_grad=True)
+    pos, inv = torch.arange(5, device=dev)[None], torch.rand(32, device=dev)
+    a, b = ops.rotary_axes(q, k, pos, inv, (32,))
+    (dk,) = torch.autograd.grad(b.sum(), k, retain_graph=True)      # an expanded gradient, and none for q
+    want = ref.rotary(torch.ones(5, 1, 64), pos.cpu(), inv.cpu(), (32,), "blocked", "half", True)
+    assert torch.allclose(dk.cpu().double(), want, atol=2.0 ** -19, rtol=0)
+    (dq,) = torch.autograd.grad(a.sum(), q)
+    assert torch.allclose(dq.cpu().double(), want.expand(5, 2, 64), atol=2.0 ** -19, rtol=0)
+
+
+# ---- append ----------------------------------------------------------------------------------------------------------
+
+def codes_of(cache):
+    return cache.cpu().double() if cache.dtype == INT8 else cache.cpu().float().double()
+
+
+def random_cache(gen, pool, heads, page, dim, code, dev, token_major=False):
+    x = torch.randn(pool, heads, page, dim, generator=gen)
+    c = (x * 31).round().clamp(-127, 127).to(INT8) if code == INT8 else (x * 100).clamp(-448, 448).to(E4M3)
+    s = 2.0 ** torch.randint(-9, -4, (pool, heads), generator=gen).float()
+    c = c.to(dev)
+    if token_major:
+        c = c.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(code)
+    return c, s.to(dev)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("page,dim,heads,token_major", [(16, 64, 3, False), (64, 128, 2, True), (256, 256, 1, False), (32, 256, 2, True)])
+def test_append(dev, dtype, code, page, dim, heads, token_major):
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(page + dim)
+    pool = 9
+    kc, ks = random_cache(gen, pool, heads, page, dim, code, dev, token_major)
+    vc, vs = random_cache(gen, pool, heads, page, dim, code, dev, token_major)
+    # runs: inside a page, up to its end, from its start, one row, a full page, skipped rows between, past the pool
+    runs = [(3, 5, 7), (5, page - 4, 4), (2, 0, 3), (-1, 0, 2), (7, page - 1, 1), (0, 0, page), (pool, 0, 3), (1, 1, 1), (8, 0, 1), (8, 1, page - 1)]
+    slots = [s for b, o, n in runs for s in ([-1] * n if b < 0 else range(b * page + o, b * page + o + n))]
+    T = len(slots)
+    size = torch.exp(torch.randn(T, 1, 1, generator=gen) * 2)
+    make = lambda: (torch.randn(T, heads, dim, generator=gen) * size).to(dtype)
+    k, v = make(), make()
+    k[0, 0] = 0
+    k[0, 0, 1] = 1e-7                    # scale stays, code rounds to 0
+    v[runs[0][2] + 4 + 1] = 0            # rows of zeros
+    k[slots.index(3 * page + 7), 1 % heads, 3:6] = torch.tensor([math.inf, -math.inf, math.nan])
+    kc2, vc2, ks2, vs2 = clone_strided(kc), clone_strided(vc), ks.clone(), vs.clone()
+    ops.paged_kv_append(k.to(dev), v.to(dev), kc2, vc2, ks2, vs2, torch.tensor(slots, device=dev))
+    for x, c, s, c2, s2, name in ((k, kc, ks, kc2, ks2, "key"), (v, vc, vs, vc2, vs2, "value")):
+        want, scale = codes_of(c), s.cpu().double()
+        ref.append(x, want, scale, slots, code)
+        assert torch.equal(s2.cpu().double(), scale), name
+        got = codes_of(c2)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num()), name
+
+
+def clone_strided(c):
+    raw = torch.empty_strided(c.shape, c.stride(), dtype=torch.uint8, device=c.device)
+    raw.copy_(c.view(torch.uint8))
+    return raw.view(c.dtype)
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+def test_append_extremes_of_scale(dev, code):
+    """All zeros (scale 0, then the first larger row), the smallest and largest fp32 magnitudes, exact powers of two times the
+    largest code and its neighbours."""
+    from fla_hip import ops
+    most = ref.LARGEST[code]
+    up = lambda x: float(torch.nextafter(torch.tensor(x), torch.tensor(math.inf)))
+    tops = [0.0, 1e-45, 2.0 ** -126, most * 2.0 ** -126, most, up(most), most * 2.0 ** 30, up(most * 2.0 ** 30), 3.4e38, 2.0, 1.0, 1.75, up(1.75), 1.984375, up(1.984375)]
+    T, page = len(tops), 16
+    x = torch.zeros(T, 1, 64)
+    x[:, 0, 0] = torch.tensor(tops)
+    x[:, 0, 1] = -torch.tensor(tops) / 3
+    slots = [t * page for t in range(T)]
+    new = lambda: torch.zeros(T, 1, page, 64, dtype=torch.uint8, device=dev).view(code)
+    kc, vc, ks, vs = new(), new(), torch.full((T, 1), 77.0, device=dev), torch.full((T, 1), 77.0, device=dev)
+    for step in range(2):                # the second row of each page comes after the first, ten times as large
+        rows = (x * 10 ** step).clamp(-3.4e38, 3.4e38)
+        ops.paged_kv_append(rows.to(dev), (-rows).to(dev), kc, vc, ks, vs, torch.tensor([s + step for s in slots], device=dev))
+        if step == 0:
+            want, scale = torch.zeros(T, 1, page, 64, dtype=torch.float64), torch.full((T, 1), 77.0, dtype=torch.float64)
+        ref.append(rows, want, scale, [s + step for s in slots], code)
+        assert torch.equal(ks.cpu().double(), scale) and torch.equal(vs.cpu().double(), scale)
+        assert torch.equal(codes_of(kc), want) and torch.equal(codes_of(vc), -want)
+
+
+# ---- attention -------------------------------------------------------------------------------------------------------
+
+def make_table(rng, lens, page, width, pool):
+    ids = list(range(pool))
+    rng.shuffle(ids)
+    table = torch.full((len(lens), width), -1, dtype=torch.int32)
+    for r, n in enumerate(lens):
+        for j in range(min(-(-n // page), width)):
+            table[r, j] = ids.pop()
+    return table
+
+
+def check_attention(dev, q, caches, table, lens, cu, scale, *, got=None, **kw):
+    from fla_hip import ops
+    kc, vc, ks, vs = caches
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    if got is None:
+        got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, table.to(dev), i32(lens), None if cu is None else i32(cu), scale=scale, return_lse=True, **kw)
+    out, lse = (t.cpu().double() for t in got)
+    want, want_lse, spread, reach = ref.attention(q, codes_of(kc), codes_of(vc), ks.cpu(), vs.cpu(), table, lens, cu, scale)
+    d = q.shape[-1]
+    score = (d + 8) * 2.0 ** -24 * reach
+    top = float(vs.max()) * ref.LARGEST[kc.dtype]
+    bound = want.abs() * torch.finfo(q.dtype).eps / 2 * 1.01 + spread * (2.0 ** -12 * 1.01 + 2 * score[..., None]) + max(lens) * 2.0 ** -25 * top + torch.finfo(q.dtype).tiny
+    assert torch.equal(out.isnan(), want.isnan())
+    error = torch.where(want.isnan(), 0.0, (out - want).abs())
+    assert bool((error <= torch.where(bound.isnan(), math.inf, bound)).all()), float((error / bound).nan_to_num().max())
+    seen = want_lse > -math.inf
+    assert torch.equal(lse > -math.inf, seen)
+    lse_error = (lse - want_lse)[seen].abs()
+    assert bool((lse_error <= score[seen] + 2.0 ** -21 * (1 + want_lse[seen].abs())).all()), float(lse_error.max())
+    return out, lse
+
+
+DECODE = [
+    # page, heads, kv heads, dim, query type, code
+    (64, 8, 2, 128, BF, E4M3), (16, 6, 1, 64, F16, INT8), (32, 4, 4, 256, BF, INT8), (128, 20, 1, 128, F16, E4M3),
+    (256, 5, 1, 64, BF, E4M3), (16, 40, 2, 256, F16, E4M3), (64, 7, 7, 128, BF, INT8)]
+
+
+@pytest.mark.parametrize("page,heads,kv_heads,dim,dtype,code", DECODE)
+def test_decode(dev, page, heads, kv_heads, dim, dtype, code):
+    rng, gen = random.Random(page + heads), torch.Generator().manual_seed(heads * dim)
+    lens = [1, 0, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 255, 256, 257, 700, 3, 1029, 8]
+    width = max(-(-n // page) for n in lens) + 2
+    pool = sum(-(-n // page) for n in lens) + 5
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, code, dev, token_major=page == 32)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, code, dev, token_major=page == 32)
+    q = torch.randn(len(lens), heads, dim, generator=gen).to(dtype)
+    out, lse = check_attention(dev, q, (kc, vc, ks, vs), make_table(rng, lens, page, width, pool), lens, None, dim ** -0.5)
+    assert bool((out[1] == 0).all()) and bool((lse[1] == -math.inf).all())
+
+
+@pytest.mark.parametrize("page,heads,kv_heads,dim,dtype,code", DECODE)
+def test_several_query_rows(dev, page, heads, kv_heads, dim, dtype, code):
+    """Ragged numbers of query rows, causal inside them; a request without any, one whose query is its whole text."""
+    rng, gen = random.Random(page), torch.Generator().manual_seed(page * dim)
+    new = [1, 4, 0, 7, 33, 70, 2, 5]
+    lens = [50, 4, 30, 300, 40, 70, 1 + 2 * page, 260]
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    width = max(-(-n // page) for n in lens)
+    pool = sum(-(-n // page) for n in lens) + 2
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, code, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, code, dev)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(dtype)
+    table = make_table(rng, lens, page, width, pool)
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, cu, dim ** -0.5, max_query_len=70)
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, cu, 0.2)
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, cu, dim ** -0.5, max_query_len=1)     # a hint that is wrong only costs time
+
+
+@pytest.mark.parametrize("lens", [[20011], [9000, 1, 0, 300], [2049, 4097, 64]])
+@pytest.mark.parametrize("code", [E4M3, INT8])
+def test_long_contexts_are_split_and_joined(dev, lens, code):
+    rng, gen = random.Random(1), torch.Generator().manual_seed(len(lens))
+    page, heads, kv_heads, dim = 64, 8, 2, 128
+    pool = sum(-(-n // page) for n in lens) + 2
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, code, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, code, dev)
+    table = make_table(rng, lens, page, max(-(-n // page) for n in lens), pool)
+    q = torch.randn(len(lens), heads, dim, generator=gen).to(BF)
+    check_attention(dev, q * 3, (kc, vc, ks, vs), table, lens, None, dim ** -0.5)
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + min(n, 3))
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(BF)
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, cu, dim ** -0.5, max_query_len=3)
+
+
+@pytest.mark.parametrize("new", [1, 5, 80])
+@pytest.mark.parametrize("page", [16, 64])
+def test_what_is_not_seen_may_hold_anything(dev, new, page):
+    """NaN codes behind the last token, in pages of nobody, in tokens that only later rows see; scales of pages of nobody
+    NaN and infinite; table entries behind the last page that name them."""
+    rng, gen = random.Random(3), torch.Generator().manual_seed(page)
+    heads, kv_heads, dim, lens = 8, 2, 128, [new + 5, new + page, new, new + 3 * page + 7]
+    pool = sum(-(-n // page) for n in lens) + 6
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    width = max(-(-n // page) for n in lens) + 3
+    table = make_table(rng, lens, page, width, pool)
+    owned = set(table[table >= 0].tolist())
+    nobody = [b for b in range(pool) if b not in owned]
+    nan = 0x7f
+    for c in (kc, vc):
+        raw = c.view(torch.uint8)
+        raw[nobody] = nan
+        for r, n in enumerate(lens):
+            if n % page:
+                raw[int(table[r, (n - 1) // page]), :, n % page:] = nan
+    for s, bad in ((ks, math.nan), (vs, math.inf), (vs, math.nan)):
+        s[nobody[::2] if bad == math.inf else nobody[1::2]] = bad
+    for r in range(len(lens)):
+        table[r, -(-lens[r] // page):] = torch.tensor([nobody[(r + j) % len(nobody)] for j in range(width - -(-lens[r] // page))])
+    cu = [new * r for r in range(len(lens) + 1)]
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(BF)
+    safe_ks, safe_vs = ks.clone(), vs.clone()
+    safe_ks[nobody] = 0
+    safe_vs[nobody] = 0
+    from fla_hip import ops
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, table.to(dev), i32(lens), i32(cu), return_lse=True)
+    check_attention(dev, q, (kc, vc, safe_ks, safe_vs), table, lens, cu, dim ** -0.5, got=got)
+    if new > 1:                            # the last token of request 0: its row sees a NaN, the others must not
+        where = int(table[0, (lens[0] - 1) // page]), (lens[0] - 1) % page
+        kc.view(torch.uint8)[where[0], :, where[1]] = nan
+        vc.view(torch.uint8)[where[0], 0, where[1], 5] = nan
+        got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, table.to(dev), i32(lens), i32(cu), return_lse=True)
+        out = got[0].cpu()
+        assert bool(out[new - 1].isnan().all()) and bool(out[:new - 1].isfinite().all()) and bool(out[new:].isfinite().all())
+        kc.view(torch.uint8)[where[0], :, where[1]] = 0x38
+        got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, table.to(dev), i32(lens), i32(cu), return_lse=True)
+        check_attention(dev, q, (kc, vc, safe_ks, safe_vs), table, lens, cu, dim ** -0.5, got=got)
+        assert bool(got[0][new - 1, :heads // kv_heads, 5].isnan().all()) and int(got[0].isnan().sum()) == heads // kv_heads
+
+
+def test_pages_outside_the_pool_are_not_seen(dev):
+    rng, gen = random.Random(4), torch.Generator().manual_seed(4)
+    page, heads, kv_heads, dim = 16, 4, 1, 64
+    lens = [100, 70, 40, 33]
+    kc, ks = random_cache(gen, 30, kv_heads, page, dim, INT8, dev)
+    vc, vs = random_cache(gen, 30, kv_heads, page, dim, INT8, dev)
+    table = make_table(rng, lens, page, 5, 30)                  # request 0 is longer than its row of the table
+    table[0, 1], table[1, 0], table[1, 3] = -1, 30, 2 ** 31 - 1
+    table[2] = -5                                                # sees nothing
+    q = torch.randn(4, heads, dim, generator=gen).to(BF)
+    out, lse = check_attention(dev, q, (kc, vc, ks, vs), table, lens, None, dim ** -0.5)
+    assert bool((out[2] == 0).all()) and bool((lse[2] == -math.inf).all())
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_scales_of_very_different_sizes(dev, new):
+    """Pages of zeros (scale 0), of tiny and of large values side by side."""
+    rng, gen = random.Random(6), torch.Generator().manual_seed(6)
+    page, heads, kv_heads, dim, lens = 16, 8, 2, 128, [333, 250]
+    pool = 60
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    vs.copy_(torch.tensor([0.0, 2.0 ** -126, 1e-30, 1e-3, 1.0, 37.0])[torch.randint(0, 6, (pool, kv_heads), generator=gen)])
+    ks[::3] = 0
+    table = make_table(rng, lens, page, 21, pool)
+    q = torch.randn(2 * new, heads, dim, generator=gen).to(BF)
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, [0, new, 2 * new], dim ** -0.5)
+    vs.fill_(2.0 ** -120)                  # fp32 holds it, the result type bf16 as well
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, [0, new, 2 * new], dim ** -0.5)
+    vs.zero_()
+    out, _ = check_attention(dev, q, (kc, vc, ks, vs), table, lens, [0, new, 2 * new], dim ** -0.5)
+    assert bool((out == 0).all())
+
+
+def test_peaked_and_far_scores(dev):
+    """Scores of a few hundred with the largest at the end, at the start, and all equal."""
+    rng, gen = random.Random(8), torch.Generator().manual_seed(8)
+    page, heads, kv_heads, dim, lens = 64, 4, 1, 64, [500, 500, 500]
+    kc, ks = random_cache(gen, 30, kv_heads, page, dim, INT8, dev)
+    vc, vs = random_cache(gen, 30, kv_heads, page, dim, INT8, dev)
+    table = make_table(rng, lens, page, 8, 30)
+    ks.fill_(2.0 ** -5)
+    first, last = int(table[0, 0]), int(table[1, 7])
+    kc[first, :, 0] = 127
+    kc[last, :, 499 % page] = 127
+    kc[table[2].long()] = 1
+    q = torch.full((3, heads, dim), 8.0).to(BF)
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, None, 1.0)
+    check_attention(dev, -q, (kc, vc, ks, vs), table, lens, None, 1.0)
+
+
+def test_given_out_keeps_the_rows_behind_the_last_request(dev):
+    from fla_hip import ops
+    rng, gen = random.Random(9), torch.Generator().manual_seed(9)
+    page, heads, kv_heads, dim, lens, cu = 16, 4, 2, 64, [20, 33], [0, 2, 5]
+    kc, ks = random_cache(gen, 9, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, 9, kv_heads, page, dim, E4M3, dev)
+    table = make_table(rng, lens, page, 3, 9)
+    q = torch.randn(9, heads, dim, generator=gen).to(BF)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    args = (q.to(dev), kc, vc, ks, vs, table.to(dev), i32(lens), i32(cu))
+    wide = torch.full((9, heads + 1, 2 * dim), 3.0, dtype=BF, device=dev)
+    out = wide[:, 1:, :dim]
+    version = wide._version
+    assert ops.paged_kv_attention(*args, out=out) is out and wide._version > version
+    new, lse = ops.paged_kv_attention(*args, return_lse=True)
+    assert torch.equal(out[:5], new[:5]) and bool((out[5:] == 3).all()) and bool((wide[:, 0] == 3).all()) and bool((wide[:, :, dim:] == 3).all())
+    assert bool((new[5:] == 0).all()) and bool((lse[5:] == -math.inf).all()) and bool(lse[:5].isfinite().all())
+    check_attention(dev, q[:5], (kc, vc, ks, vs), table, lens, cu, dim ** -0.5, got=(new[:5], lse[:5]))
+
+
+def test_cache_beyond_32_bit_offsets(dev):
+    """Pages whose codes lie past 2^32 bytes."""
+    from fla_hip import ops
+    page, heads, kv_heads, dim = 64, 4, 8, 128
+    pool = (1 << 32) // (page * kv_heads * dim) + 40
+    caches = [torch.empty(pool, kv_heads, page, dim, dtype=torch.uint8, device=dev).view(E4M3) for _ in range(2)]
+    scales = [torch.zeros(pool, kv_heads, device=dev) for _ in range(2)]
+    gen = torch.Generator().manual_seed(1)
+    lens, n = [150], 150
+    table = torch.tensor([[pool - 1, 3, pool - 7]], dtype=torch.int32)
+    slots = torch.tensor([int(table[0, t // page]) * page + t % page for t in range(n)], device=dev)
+    k, v = torch.randn(n, kv_heads, dim, generator=gen).to(BF), torch.randn(n, kv_heads, dim, generator=gen).to(BF)
+    ops.paged_kv_append(k.to(dev), v.to(dev), *caches, *scales, slots)
+    q = torch.randn(1, 8 * 4, dim, generator=gen).to(BF)
+    got = ops.paged_kv_attention(q.to(dev), *caches, *scales, table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), return_lse=True)
+    used = table[0].long()
+    small = [c.view(torch.uint8)[used.to(dev)].view(E4M3) for c in caches] + [s[used.to(dev)] for s in scales]
+    check_attention(dev, q, small, torch.tensor([[0, 1, 2]], dtype=torch.int32), lens, None, dim ** -0.5, got=got)
+
+
+# ---- together --------------------------------------------------------------------------------------------------------
+
+def serve(dev, steps, code, capture, side_stream=False):
+    """A batch served for several steps: plan, rotary, append, attention; every step against the restatement."""
+    from fla_hip import ops
+    gen, rng = torch.Generator().manual_seed(11), random.Random(11)
+    page, heads, kv_heads, dim, pool, n, width, T = 16, 8, 2, 64, 64, 4, 10, steps[0][1]
+    new = lambda: torch.zeros(pool, kv_heads, page, dim, dtype=torch.uint8, device=dev).view(code)
+    kc, vc, ks, vs = new(), new(), torch.zeros(pool, kv_heads, device=dev), torch.zeros(pool, kv_heads, device=dev)
+    table = torch.full((n, width), -1, dtype=torch.int32, device=dev)
+    ids = list(range(pool))
+    rng.shuffle(ids)
+    inv = (10000.0 ** (-torch.arange(16) / 16)).to(dev)
+    buf = dict(context=torch.zeros(n, dtype=torch.int32, device=dev), query=torch.zeros(n, dtype=torch.int32, device=dev),
+               free=torch.zeros(16, dtype=torch.int32, device=dev), q=torch.zeros(T, heads, dim, dtype=BF, device=dev),
+               k=torch.zeros(T, kv_heads, dim, dtype=BF, device=dev), v=torch.zeros(T, kv_heads, dim, dtype=BF, device=dev))
+
+    def step():
+        slots, pos, cu, seq, used, _ = ops.paged_kv_plan(buf["context"], buf["query"], table, buf["free"], page, T)
+        q, k = ops.rotary_axes(buf["q"], buf["k"], pos[None].expand(2, -1), inv, (8, 8), axis_order="interleaved")
+        ops.paged_kv_append(k, buf["v"], kc, vc, ks, vs, slots)
+        return q, k, slots, cu, seq, used, ops.paged_kv_attention(q, kc, vc, ks, vs, table, seq, cu, max_query_len=T, return_lse=True)
+
+    graph = None
+    if capture:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            static = step()
+        for t in (kc, vc):
+            t.view(torch.uint8).zero_()
+        ks.zero_()
+        vs.zero_()
+        table.fill_(-1)
+    context, at = [0] * n, 0
+    ref_table = [[-1] * width for _ in range(n)]
+    state = [torch.zeros(pool, kv_heads, page, dim, dtype=torch.float64) for _ in range(2)] + [torch.zeros(pool, kv_heads, dtype=torch.float64) for _ in range(2)]
+    for query, tokens in steps:
+        assert tokens == T
+        free = ids[at:at + 16]
+        buf["context"].copy_(torch.tensor(context))
+        buf["query"].copy_(torch.tensor(query))
+        buf["free"][:len(free)] = torch.tensor(free, dtype=torch.int32, device=dev)
+        for name in "qkv":
+            buf[name].copy_(torch.randn(buf[name].shape, generator=gen) * (1 + sum(context)))
+        if side_stream:
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                q, k, slots, cu, seq, used, got = step()
+            torch.cuda.current_stream().wait_stream(stream)
+        elif graph is not None:
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            q, k, slots, cu, seq, used, got = static
+        else:
+            q, k, slots, cu, seq, used, got = step()
+        want = ref.plan(context, query, ref_table, free, page, T)
+        assert torch.equal(slots.cpu(), want["slots"]) and torch.equal(table.cpu(), want["table"]) and torch.equal(used.cpu(), want["used"])
+        total = sum(query)
+        ref.append(k.cpu(), state[0], state[2], want["slots"], code)
+        ref.append(buf["v"].cpu(), state[1], state[3], want["slots"], code)
+        assert torch.equal(ks.cpu().double(), state[2]) and torch.equal(vs.cpu().double(), state[3])
+        assert torch.equal(codes_of(kc), state[0]) and torch.equal(codes_of(vc), state[1])
+        out, lse = (t[:total] for t in got)
+        assert bool((got[0][total:] == 0).all())
+        check_attention(dev, q[:total].cpu(), (kc, vc, ks, vs), table.cpu(), seq.tolist(), cu.tolist(), dim ** -0.5, got=(out, lse))
+        context = [c + m for c, m in zip(context, query)]
+        at += int(used)
+
+
+PREFILL = [([17, 5, 0, 10], 32)]
+STEPS = [([3, 1, 20, 1], 32), ([1, 1, 1, 1], 32), ([0, 16, 1, 2], 32), ([1, 0, 1, 30], 32)]
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("way", ["eager", "graph", "stream"])
+def test_plan_rotary_append_attention_together(dev, code, way):
+    serve(dev, PREFILL + STEPS, code, way == "graph", way == "stream")
+
+
+def test_plan_feeds_the_recurrent_operator(dev):
+    """The plan's state rows and lengths drive recurrent_gated_delta_rule on its state pool, as one step of a hybrid stack."""
+    from fla_hip import ops
+    import torch.nn.functional as F
+    gen = torch.Generator().manual_seed(2)
+    lens, D, H, rows = [2, 1, 3], 64, 2, [4, 0, 6]
+    T = sum(lens)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    with_lead = i32([0] + lens)                 # the recurrent operator's lengths; the plan takes the same buffer without the lead
+    *_, states = ops.paged_kv_plan(i32([5, 0, 9]), with_lead[1:], torch.full((3, 2), -1, dtype=torch.int32, device=dev), i32([1, 2, 3, 4]), 16, T, state_rows=i32(rows))
+    assert states.tolist() == [r for r, n in zip(rows, lens) for _ in range(n)]
+    rn = lambda *s: torch.randn(*s, generator=gen)
+    q, k, v = (F.normalize(rn(T, H, D), dim=-1).to(BF).to(dev) for _ in range(3))
+    beta, g = torch.sigmoid(rn(T, H)).to(BF).to(dev), F.logsigmoid(rn(T, H)).to(dev)
+    pool = (rn(8, H, D, D) * 0.01).to(dev)
+    expect_pool = pool.clone()
+    kw = dict(beta=beta, scale=D ** -0.5, actual_seq_lengths=with_lead, g=g)
+    o = ops.recurrent_gated_delta_rule(q, k, v, pool, ssm_state_indices=states, **kw)
+    e = ops.recurrent_gated_delta_rule(q, k, v, expect_pool, ssm_state_indices=i32([4, 4, 0, 6, 6, 6]), **kw)
+    assert torch.equal(o, e) and torch.equal(pool, expect_pool)
+
+
+def test_refusals_of_gradients_and_cpu_tensors(dev):
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(0)
+    kc, ks = random_cache(gen, 4, 1, 16, 64, E4M3, dev)
+    q = torch.randn(1, 2, 64, device=dev, dtype=BF, requires_grad=True)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    with pytest.raises(NotImplementedError, match="no gradient is bound for query"):
+        ops.paged_kv_attention(q, kc, kc, ks, ks, table, lens)
+    with torch.no_grad():
+        ops.paged_kv_attention(q, kc, kc, ks, ks, table, lens)
+    with torch.inference_mode():
+        ops.paged_kv_attention(q, kc, kc, ks, ks, table, lens, out=torch.empty(1, 2, 64, device=dev, dtype=BF))
+    with pytest.raises(TypeError, match="key_cache must be a ROCm GPU tensor"):
+        ops.paged_kv_attention(q.detach(), kc.cpu(), kc, ks, ks, table, lens)
