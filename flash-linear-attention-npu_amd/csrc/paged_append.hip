@@ -25,7 +25,7 @@ struct AppendParams {
     AppendSide side[2];
     const int64_t *slots;
     int64_t tokens, pool;
-    int shift, heads, dim, tokens_per_wg;
+    int shift, heads, dim, row_shift, tokens_per_wg;   // row_shift: log2 of the 8-element pieces of a row
 };
 
 // smallest power of two s >= 2^-126 with a / s <= most; 0 for a = 0.  a >= 0 and finite.
@@ -38,24 +38,7 @@ template <int CODE> __device__ __forceinline__ float step_for(float a) {
     return a == 0.f ? 0.f : __builtin_bit_cast(float, (unsigned)max(e, 1) << 23);
 }
 
-// four values (already divided by the scale) as four codes
-template <int CODE> __device__ __forceinline__ unsigned encode4(float a, float b, float c, float d) {
-    float v[4] = {a, b, c, d};
-    if constexpr (CODE == FLA_I8) {
-        unsigned r = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float t = v[e] == v[e] ? __builtin_amdgcn_fmed3f(v[e], -127.f, 127.f) : 0.f;
-            r |= ((unsigned)(int)rintf(t) & 255u) << (8 * e);
-        }
-        return r;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = v[e] == v[e] ? __builtin_amdgcn_fmed3f(v[e], -448.f, 448.f) : v[e];
-        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-        return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
-    }
-}
+// Codes as numbers.
 template <int CODE> __device__ __forceinline__ void decode4(unsigned x, float (&v)[4]) {
     if constexpr (CODE == FLA_I8) {
 #pragma unroll
@@ -69,54 +52,148 @@ template <int CODE> __device__ __forceinline__ void decode4(unsigned x, float (&
     }
 }
 
-// division by a scale: a power of two (every scale this operator writes) takes an exact product
-struct Divide {
-    float by, inv;
-    bool exact;
-    __device__ __forceinline__ explicit Divide(float s)
-        : by(s), inv(s > 0.f ? 1.f / s : 0.f), exact((__builtin_bit_cast(unsigned, s) & 0x7fffffu) == 0) {}
-    __device__ __forceinline__ float operator()(float x) const { return exact || by == 0.f ? x * inv : x / by; }
+// Four values, already divided by the scale and inside the range of the codes, as four codes, rounded to nearest even.
+template <int CODE> __device__ __forceinline__ unsigned encode4(const float (&v)[4]) {
+    if constexpr (CODE == FLA_I8) {
+        // 1.5 * 2^23 + v: the sum rounds v to an integer, whose two's complement is the low byte
+        unsigned u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = __builtin_bit_cast(unsigned, v[e] + 12582912.f);
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u), __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), 0x05040100u);
+    } else {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+    }
+}
+// Infinities to the largest code; NaN stays (e4m3) or turns into 0 (int8).
+template <int CODE> __device__ __forceinline__ float into_range(float v) {
+    constexpr float kMost = CODE == FLA_I8 ? 127.f : 448.f;
+    return v == v ? __builtin_amdgcn_fmed3f(v, -kMost, kMost) : CODE == FLA_I8 ? 0.f : v;
+}
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// Running maximum of magnitudes as bit patterns (magnitudes order like them): two 16-bit values to a dword, or one fp32.
+template <typename T> __device__ __forceinline__ unsigned max_bits(unsigned a, unsigned x) {
+    if constexpr (sizeof(T) == 2)
+        return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, x & 0x7fff7fffu)));
+    else
+        return max(a, x & 0x7fffffffu);
+}
+// fp32 magnitude of the larger half (or of the fp32 pattern); infinite or NaN if any element was
+template <typename T> __device__ __forceinline__ float magnitude(unsigned bits) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, bits);
+    else return to_f32(__builtin_bit_cast(T, (unsigned short)max(bits & 0xffffu, bits >> 16)));
+}
+
+template <typename T> struct Piece8 {                 // eight elements
+    static constexpr int kWords = sizeof(T) * 2;
+    unsigned w[kWords];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
+            const u32x4 v = reinterpret_cast<const u32x4 *>(p)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[e]);
+        else if constexpr (__is_same(T, bf16)) return __builtin_bit_cast(float, (e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        else return to_f32(__builtin_bit_cast(T, (unsigned short)((e & 1) ? w[e >> 1] >> 16 : w[e >> 1])));
+    }
 };
 
-constexpr int kPieces = 8;   // 8-element pieces a thread holds
+template <int CODE, typename F> __device__ __forceinline__ void store_piece(uint8_t *at, F &&value) {
+    u32x2 code;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = value(4 * half + e);
+        code[half] = encode4<CODE>(v);
+    }
+    *reinterpret_cast<u32x2 *>(at) = code;
+}
+
+__device__ __forceinline__ int ones(uint64_t x) { return ~x ? (int)__ffsll((unsigned long long)~x) - 1 : 64; }   // trailing ones
+
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {   // of a wave-uniform lane, into scalar registers
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)v, lane), hi = __builtin_amdgcn_readlane((unsigned)(v >> 32), lane);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// pieces of eight elements that a thread holds
+template <typename T> constexpr int pieces_held() { return sizeof(T) == 2 ? 16 : 8; }
 
 template <typename T, int CODE, int W>
 __global__ void __launch_bounds__(W * 64) paged_kv_append_kernel(const AppendParams p) {
-    constexpr int kThreads = W * 64;
-    typedef T T8 __attribute__((ext_vector_type(8)));
+    constexpr int kThreads = W * 64, kHeld = pieces_held<T>();
     __shared__ float wave_max[W];
-    __shared__ int run_end;
     const int tid = threadIdx.x, lane = tid & 63;
     const AppendSide s = p.side[blockIdx.z];
-    const int head = blockIdx.y, page = 1 << p.shift, ppr = p.dim >> 3;   // 8-element pieces per row
-    const int64_t first = (int64_t)blockIdx.x * p.tokens_per_wg, last = min(first + p.tokens_per_wg, p.tokens);
-    for (int64_t t = first; t < last; ++t) {
-        const int64_t slot = p.slots[t], block = slot >> p.shift;
-        if (slot < 0 || block >= p.pool) continue;
+    const int head = blockIdx.y, page = 1 << p.shift, row_shift = p.row_shift, row_mask = (1 << row_shift) - 1;
+    const int64_t first = (int64_t)blockIdx.x * p.tokens_per_wg;
+    const int count = (int)min((int64_t)p.tokens_per_wg, p.tokens - first);
+    // the slots of tokens first - 1 + lane and first + 63 + lane: the runs that begin here (at most 32 tokens) and nearly
+    // always their ends.  Bit w of (lo, hi): token first - 1 + w continues the run of the one before it.
+    const int64_t at = first - 1 + lane;
+    const int64_t mine = at >= 0 && at < p.tokens ? p.slots[at] : -2, more = at + 64 < p.tokens ? p.slots[at + 64] : -2;
+    const int64_t prev = __shfl_up(mine, 1, kWave), last = __shfl(mine, 63, kWave), up = __shfl_up(more, 1, kWave);
+    const int64_t prev_more = lane ? up : last;
+    const bool follows = lane >= 1 && prev >= 0 && mine == prev + 1 && (mine & (page - 1)) != 0;
+    const uint64_t lo = __ballot(follows), hi = __ballot(prev_more >= 0 && more == prev_more + 1 && (more & (page - 1)) != 0);
+    uint64_t starts = __ballot(lane >= 1 && lane <= count && mine >= 0 && (mine >> p.shift) < p.pool && !follows);
+    while (starts) {
+        const int l = __ffsll((unsigned long long)starts) - 1;
+        starts &= starts - 1;
+        const int64_t t = first + l - 1, slot = lane_value(mine, l), block = slot >> p.shift;
         const int off = (int)(slot & (page - 1));
-        if (off > 0 && t > 0 && p.slots[t - 1] == slot - 1) continue;   // not the first row of its run
-        // rows of the run: while the slots ascend one by one inside the page
-        if (tid == 0) run_end = page - off;
-        __syncthreads();
-        for (int i = tid + 1; i < page - off; i += kThreads)
-            if (t + i >= p.tokens || p.slots[t + i] != slot + i) atomicMin(&run_end, i);
-        __syncthreads();
-        const int rows = run_end, pieces = rows * ppr;
-        const T *x = static_cast<const T *>(s.x) + t * s.x_t + head * s.x_h;
-        T8 held[kPieces];
-        float most = 0.f;
-#pragma unroll
-        for (int m = 0; m < kPieces; ++m) {
-            const int i = tid + m * kThreads;
-            if (i < pieces) {
-                const int row = i / ppr;
-                held[m] = *reinterpret_cast<const T8 *>(x + row * s.x_t + (i - row * ppr) * 8);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float a = fabsf(to_f32(held[m][e]));
-                    most = fmaxf(most, a < INFINITY ? a : 0.f);
-                }
+        int rows = 1 + ones(lo >> (l + 1));                                       // zeros shift in behind bit 63
+        if (rows == 64 - l) {
+            rows += ones(hi);
+            while (rows >= 128 - l && off + rows < page) {                        // pages of 128 or 256
+                const int64_t u = t + rows + lane;
+                const int n = ones(__ballot(u < p.tokens && p.slots[min(u, p.tokens - 1)] == slot + rows + lane));
+                rows += n;
+                if (n < 64) break;
             }
+            rows = min(rows, page - off);
+        }
+        const int pieces = rows << row_shift;
+        const T *x = static_cast<const T *>(s.x) + t * s.x_t + head * s.x_h;
+        const unsigned x_t = (unsigned)s.x_t, c_t = (unsigned)s.c_t;              // rows of a page: 32-bit offsets
+        float *scale = s.scales + block * s.s_p + head * s.s_h;
+        const float before = off > 0 ? *scale : 0.f;
+        Piece8<T> held[kHeld];
+        unsigned bits = 0;
+#pragma unroll
+        for (int m = 0; m < kHeld; ++m) {
+            const int i = tid + m * kThreads;
+            if (m == 0 || m * kThreads < pieces) {
+                const int j = min(i, pieces - 1);                                 // a piece too many is read twice
+                held[m].load(x + ((unsigned)(j >> row_shift) * x_t + (j & row_mask) * 8));
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < kHeld; ++m)
+            if (m == 0 || m * kThreads < pieces) {
+#pragma unroll
+                for (int w = 0; w < Piece8<T>::kWords; ++w) bits = max_bits<T>(bits, held[m].w[w]);
+            }
+        float most = magnitude<T>(bits);
+        bool odd = !(most < INFINITY);
+        if (__any(odd)) {                                                         // infinities or NaN: the maximum of the others
+            most = 0.f;
+#pragma unroll
+            for (int m = 0; m < kHeld; ++m)
+                if (m * kThreads < pieces) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float a = fabsf(held[m].get(e));
+                        most = fmaxf(most, a < INFINITY ? a : 0.f);
+                    }
+                }
         }
 #pragma unroll
         for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d, kWave));
@@ -126,49 +203,53 @@ __global__ void __launch_bounds__(W * 64) paged_kv_append_kernel(const AppendPar
 #pragma unroll
             for (int w = 0; w < W; ++w) most = fmaxf(most, wave_max[w]);
         }
-        float *scale = s.scales + block * s.s_p + head * s.s_h;
-        const float before = off > 0 ? *scale : 0.f, after = fmaxf(before, step_for<CODE>(most));
+        const float after = fmaxf(before, step_for<CODE>(most));
         uint8_t *cache = static_cast<uint8_t *>(s.cache) + block * s.c_p + head * s.c_h;
         if (after > before) {
             const float ratio = before / after;
-            for (int i = tid; i < off * ppr; i += kThreads) {   // earlier codes to the new scale
-                const int row = i / ppr;
-                u32x2 *at = reinterpret_cast<u32x2 *>(cache + row * s.c_t + (i - row * ppr) * 8);
-                u32x2 code = *at;
+            for (int i = tid; i < off << row_shift; i += kThreads) {              // earlier codes to the new scale
+                u32x2 *to = reinterpret_cast<u32x2 *>(cache + ((unsigned)(i >> row_shift) * c_t + (i & row_mask) * 8));
+                u32x2 code = *to;
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                     float v[4];
                     decode4<CODE>(code[w], v);
-                    code[w] = encode4<CODE>(v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] *= ratio;
+                    code[w] = encode4<CODE>(v);
                 }
-                *at = code;
+                *to = code;
             }
         }
-        const Divide div(after);
+        // a power of two (every scale this operator writes): an exact product; another scale from outside: a division
+        const bool exact = (__builtin_bit_cast(unsigned, after) & 0x7fffffu) == 0;
+        const float inv = after > 0.f ? 1.f / after : 0.f;
+        const bool plain = exact && !__any(odd);
 #pragma unroll
-        for (int m = 0; m < kPieces; ++m) {
+        for (int m = 0; m < kHeld; ++m) {
             const int i = tid + m * kThreads;
             if (i < pieces) {
-                const int row = i / ppr;
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = div(to_f32(held[m][e]));
-                const u32x2 code = {encode4<CODE>(v[0], v[1], v[2], v[3]), encode4<CODE>(v[4], v[5], v[6], v[7])};
-                *reinterpret_cast<u32x2 *>(cache + (off + row) * s.c_t + (i - row * ppr) * 8) = code;
+                uint8_t *to = cache + ((unsigned)(off + (i >> row_shift)) * c_t + (i & row_mask) * 8);
+                if (plain) store_piece<CODE>(to, [&](int e) { return held[m].get(e) * inv; });
+                else store_piece<CODE>(to, [&](int e) { return into_range<CODE>(exact ? held[m].get(e) * inv : held[m].get(e) / after); });
             }
         }
-        __syncthreads();   // every thread has read the old scale and run_end
+        if (W > 1) __syncthreads();                                               // every wave has read the old scale
         if (tid == 0) *scale = after;
     }
 }
 
-template <typename T, int CODE> int launch(const AppendParams &p, hipStream_t stream) {
-    const int64_t unit = ((int64_t)p.dim << p.shift) / 8;   // pieces of a full page
+template <typename T, int CODE> int launch(AppendParams &p, hipStream_t stream) {
+    const int64_t unit = ((int64_t)p.dim << p.shift) / 8 / pieces_held<T>();      // threads that hold a full page
+    // Tokens per workgroup: as many as leave about 16384 workgroups, so that a decode step gets one for each row and a
+    // prefill few that find no first row (110 k tokens, 8 heads of 128, pages of 64: 1 token XX us, 32 tokens XX us).
+    p.tokens_per_wg = 1;
+    while (p.tokens_per_wg < 32 && p.tokens * p.heads * 2 >= (int64_t)16384 * 2 * p.tokens_per_wg) p.tokens_per_wg *= 2;
     const dim3 grid((unsigned)((p.tokens + p.tokens_per_wg - 1) / p.tokens_per_wg), (unsigned)p.heads, 2);
 #define FLA_APPEND(W) FLA_LAUNCH("paged_kv_append", stream, (paged_kv_append_kernel<T, CODE, W>), grid, dim3(W * 64), 0, stream, p)
-    if (unit <= 64 * kPieces) FLA_APPEND(1);
-    else if (unit <= 256 * kPieces) FLA_APPEND(4);
-    else FLA_APPEND(16);
+    if (unit <= 64) FLA_APPEND(1);
+    else if (unit <= 256) FLA_APPEND(4);
+    else FLA_APPEND((sizeof(T) == 2 ? 8 : 16));
 #undef FLA_APPEND
     FLA_HIP_CHECK(hipGetLastError());
     return FLA_OK;
@@ -189,6 +270,9 @@ int append_impl(const fla_tensor *key, const fla_tensor *value, const fla_tensor
         FLA_REQUIRE(inner_unit(x[i]) && x[i]->stride[0] >= 0 && x[i]->stride[1] >= 0 && x[i]->stride[0] % 8 == 0 && x[i]->stride[1] % 8 == 0 &&
                         reinterpret_cast<uintptr_t>(x[i]->data) % 16 == 0,
                     FLA_ERR_SHAPE, "%s: rows of %s must be contiguous and 16-byte aligned.", op, i ? "value" : "key");
+        // rows of a page are addressed with 32-bit offsets
+        FLA_REQUIRE(x[i]->stride[0] < ((int64_t)1 << 21) && cache[i]->stride[2] < ((int64_t)1 << 23), FLA_ERR_UNSUPPORTED,
+                    "%s: tokens of %s or its cache lie too far apart.", op, i ? "value" : "key");
         AppendSide &s = p.side[i];
         s.x = x[i]->data;
         s.x_t = x[i]->stride[0];
@@ -211,7 +295,7 @@ int append_impl(const fla_tensor *key, const fla_tensor *value, const fla_tensor
     p.dim = (int)shape.dim;
     if (p.tokens == 0) return FLA_OK;
     FLA_REQUIRE(p.tokens < ((int64_t)1 << 31), FLA_ERR_SHAPE, "%s: too many tokens.", op);
-    p.tokens_per_wg = 16;
+    p.row_shift = __builtin_ctz((unsigned)p.dim / 8);
 #define FLA_BY_TYPE(CODE)                                                                \
     (key->dtype == FLA_BF16 ? launch<bf16, CODE>(p, stream) : key->dtype == FLA_F16 ? launch<f16, CODE>(p, stream) : launch<float, CODE>(p, stream))
     return shape.code == FLA_I8 ? FLA_BY_TYPE(FLA_I8) : FLA_BY_TYPE(FLA_F8E4M3);
