@@ -7,7 +7,10 @@
 // page filled token by token does not drift.
 // Bound by HBM for a prefill, by latency for a decode step.  The rows of one page (a run: ascending slots) and one head
 // of k or v are a unit of W waves: the rows pass through registers once (maximum, then codes), 16 bytes per load.  A
-// workgroup looks for the first rows of runs among a few tokens; a run belongs to the workgroup of its first row.
+// workgroup looks for the first rows of runs among a few tokens (slots in lanes, runs as bit masks); a run belongs to the
+// workgroup of its first row.  Maxima are taken on the bit patterns, two 16-bit elements an instruction.
+// Measured: 110 k tokens of 8 heads of 128, pages of 64: 134 us for 679 MB = 5.1 TB/s, the rate of a copy; 256 single
+// rows: 5.7 us.
 #include "common.h"
 #include "paged_cache.h"
 
@@ -241,10 +244,11 @@ __global__ void __launch_bounds__(W * 64) paged_kv_append_kernel(const AppendPar
 
 template <typename T, int CODE> int launch(AppendParams &p, hipStream_t stream) {
     const int64_t unit = ((int64_t)p.dim << p.shift) / 8 / pieces_held<T>();      // threads that hold a full page
-    // Tokens per workgroup: as many as leave about 16384 workgroups, so that a decode step gets one for each row and a
-    // prefill few that find no first row (110 k tokens, 8 heads of 128, pages of 64: 1 token XX us, 32 tokens XX us).
+    // Tokens per workgroup: as many as leave about 8192 workgroups, so that a decode step gets one for each row and a
+    // prefill few that find no first row (110 k tokens, 8 heads of 128, pages of 64: 1 token 491 us, 4 195 us, 16 or 32
+    // 135 us; 256 single rows: 1 to 8 tokens alike, 32 tokens twice the time).
     p.tokens_per_wg = 1;
-    while (p.tokens_per_wg < 32 && p.tokens * p.heads * 2 >= (int64_t)16384 * 2 * p.tokens_per_wg) p.tokens_per_wg *= 2;
+    while (p.tokens_per_wg < 32 && p.tokens * p.heads * 2 >= (int64_t)8192 * 2 * p.tokens_per_wg) p.tokens_per_wg *= 2;
     const dim3 grid((unsigned)((p.tokens + p.tokens_per_wg - 1) / p.tokens_per_wg), (unsigned)p.heads, 2);
 #define FLA_APPEND(W) FLA_LAUNCH("paged_kv_append", stream, (paged_kv_append_kernel<T, CODE, W>), grid, dim3(W * 64), 0, stream, p)
     if (unit <= 64) FLA_APPEND(1);

@@ -27,6 +27,7 @@ struct AttnParams {
     int tokens, n, width, shift, group, heads;
     uint32_t pool;
     int target, min_units;         // items wanted; shortest chunk in units; target 0: one chunk for each tile
+    int tiles_each;                // tiles of a request without cu
     float scale2;                  // scale * log2(e)
     bool clear_tail;
 };
@@ -57,110 +58,95 @@ struct Item {
     bool found;
 };
 
-template <int THREADS> __device__ __forceinline__ int64_t block_sum64(int64_t v, int64_t *sums) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        const int lo = __shfl_xor((int)(v & 0xffffffff), d, kWave), hi = __shfl_xor((int)(v >> 32), d, kWave);
-        v += ((int64_t)hi << 32) | (uint32_t)lo;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / kWave; ++w) total += sums[w];
-    return total;
+// Inclusive prefix sum over the 64 lanes of a wave, as wave_inclusive_scan.
+__device__ __forceinline__ int wave_scan(int v) {
+#define FLA_DPP_IADD(ctrl, row_mask) v += __builtin_amdgcn_update_dpp(0, v, (ctrl), (row_mask), 0xf, true)
+    FLA_DPP_IADD(0x111, 0xf);
+    FLA_DPP_IADD(0x112, 0xf);
+    FLA_DPP_IADD(0x114, 0xf);
+    FLA_DPP_IADD(0x118, 0xf);
+    FLA_DPP_IADD(0x142, 0xa);
+    FLA_DPP_IADD(0x143, 0xc);
+#undef FLA_DPP_IADD
+    return v;
 }
 
-// Scratch of find_item in LDS.
-template <int THREADS> struct ScheduleLds {
-    int64_t sums[THREADS / kWave];
-    int wave_items[THREADS / kWave];
-    Item item;
-    int64_t base;
-};
-
-// chunk length in units
-template <int THREADS, int ROWS> __device__ __forceinline__ int chunk_units(const AttnParams &p, ScheduleLds<THREADS> &lds) {
-    if (p.target == 0) return INT32_MAX;
-    int64_t work = 0;
-    for (int r = threadIdx.x; r < p.n; r += THREADS) {
-        const Request q = request_of(p, r);
-        work += (int64_t)((q.rows + ROWS - 1) / ROWS) * q.units;
+// The item with number `want`, or (by_tile) the first item of the tile with number `want` and, in base, its number.  Every
+// wave finds it for itself, 64 requests at a time, with no LDS and no barrier: this stands before the first load of codes.
+template <int ROWS> __device__ __forceinline__ Item find_item(const AttnParams &p, int want, bool by_tile, int &base) {
+    Item it;
+    it.chunk = 0;
+    it.chunks = 1;
+    it.units = INT32_MAX;
+    if (p.target == 0 && p.cu == nullptr) {            // decode, one chunk for each request
+        it.r = want / p.tiles_each;
+        it.tile = want - it.r * p.tiles_each;
+        it.found = it.r < p.n;
+        base = want;
+        return it;
     }
-    work = block_sum64<THREADS>(work, lds.sums);
-    const int64_t c = (work + p.target - 1) / p.target;
-    return (int)min(max(c, (int64_t)p.min_units), (int64_t)INT32_MAX);
-}
-
-// The item with number `want`, or (by_tile) the first item of the tile with number `want` and, in base, its number.
-template <int THREADS, int ROWS>
-__device__ __forceinline__ Item find_item(const AttnParams &p, int64_t want, bool by_tile, ScheduleLds<THREADS> &lds, int64_t &base) {
-    const int units = chunk_units<THREADS, ROWS>(p, lds);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) lds.item.found = false;
-    int64_t items_before = 0, tiles_before = 0;
-    for (int r0 = 0; r0 < p.n; r0 += THREADS) {
-        const int r = r0 + threadIdx.x;
-        int tiles = 0, chunks = 0;
-        if (r < p.n) {
+    const int lane = threadIdx.x & 63;
+    int tiles0 = 0, units0 = 0;                         // of request `lane`
+    if (lane < p.n) {
+        const Request q = request_of(p, lane);
+        tiles0 = (q.rows + ROWS - 1) / ROWS;
+        units0 = q.units;
+    }
+    if (p.target) {
+        int64_t work = (int64_t)tiles0 * units0;
+        for (int r = lane + kWave; r < p.n; r += kWave) {
             const Request q = request_of(p, r);
-            tiles = (q.rows + ROWS - 1) / ROWS;
-            chunks = q.units <= units ? 1 : (q.units + units - 1) / units;
+            work += (int64_t)((q.rows + ROWS - 1) / ROWS) * q.units;
         }
-        const int items = tiles * chunks;
-        int inc = items, inc_t = tiles;
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-            const int up = __shfl_up(inc, d, kWave), up_t = __shfl_up(inc_t, d, kWave);
-            if (lane >= d) {
-                inc += up;
-                inc_t += up_t;
-            }
-        }
-        __syncthreads();
-        if (lane == 63) {
-            lds.wave_items[wave] = inc;
-            lds.sums[wave] = inc_t;
-        }
-        __syncthreads();
-        int64_t at = items_before + inc - items, at_t = tiles_before + inc_t - tiles;
-#pragma unroll
-        for (int w = 0; w < THREADS / kWave; ++w) {
-            if (w < wave) {
-                at += lds.wave_items[w];
-                at_t += lds.sums[w];
-            }
-            items_before += lds.wave_items[w];
-            tiles_before += lds.sums[w];
-        }
-        const int64_t mine = by_tile ? at_t : at, count = by_tile ? tiles : items;
-        if (want >= mine && want < mine + count) {
-            const int64_t k = want - mine;
-            Item it;
-            it.r = r;
-            it.tile = (int)(by_tile ? k : k / chunks);
-            it.chunk = by_tile ? 0 : (int)(k - (int64_t)it.tile * chunks);
-            it.chunks = chunks;
-            it.units = units;
-            it.found = true;
-            lds.item = it;
-            lds.base = at + (int64_t)it.tile * chunks;
-        }
-        if (want < (by_tile ? tiles_before : items_before)) break;
+        // sum over the lanes in two halves; one more than the quotient, so that rounding cannot make more items than the grid
+        const int lo = __builtin_amdgcn_readlane(wave_scan((int)(work & 0xffff)), 63), hi = __builtin_amdgcn_readlane(wave_scan((int)(work >> 16)), 63);
+        const float all = (float)hi * 65536.f + (float)lo;
+        it.units = max((int)fminf(all / (float)p.target, 1e9f) + 1, p.min_units);
     }
-    __syncthreads();
-    base = lds.base;
-    return lds.item;
+    int items_before = 0, tiles_before = 0;
+    for (int r0 = 0; r0 < p.n; r0 += kWave) {
+        int tiles = tiles0, units = units0;
+        if (r0) {
+            tiles = units = 0;
+            if (r0 + lane < p.n) {
+                const Request q = request_of(p, r0 + lane);
+                tiles = (q.rows + ROWS - 1) / ROWS;
+                units = q.units;
+            }
+        }
+        const int chunks = units <= it.units ? 1 : (units + it.units - 1) / it.units, items = tiles * chunks;
+        const int end_i = items_before + wave_scan(items), end_t = tiles_before + wave_scan(tiles);
+        const uint64_t past = __ballot((by_tile ? end_t : end_i) > want);        // the sums ascend: its request is the first one past it
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            it.r = r0 + l;
+            it.chunks = __builtin_amdgcn_readlane(chunks, l);
+            const int first_i = __builtin_amdgcn_readlane(end_i - items, l), first_t = __builtin_amdgcn_readlane(end_t - tiles, l);
+            if (by_tile) {
+                it.tile = want - first_t;
+            } else {
+                it.tile = (want - first_i) / it.chunks;
+                it.chunk = want - first_i - it.tile * it.chunks;
+            }
+            base = first_i + it.tile * it.chunks;
+            it.found = true;
+            return it;
+        }
+        items_before = __builtin_amdgcn_readlane(end_i, 63);
+        tiles_before = __builtin_amdgcn_readlane(end_t, 63);
+    }
+    it.found = false;
+    return it;
 }
 
 // ---- codes to 16-bit operands ------------------------------------------------------------------------------------
 typedef f16 f16x2v __attribute__((ext_vector_type(2)));
+constexpr float kNegInf = -__builtin_inff();
 
 // codes 2*PAIR and 2*PAIR + 1 of a dword as two bf16 or f16, both exact
 template <int CODE, typename T, int PAIR> __device__ __forceinline__ unsigned widen2(unsigned x) {
     if constexpr (CODE == FLA_F8E4M3) {
-        if constexpr (sizeof(T) == 2 && __is_same(T, bf16)) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, PAIR == 1));
+        if constexpr (__is_same(T, bf16)) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, PAIR == 1));
         else return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.f, PAIR == 1));
     } else {
         const float a = (float)(signed char)(x >> (16 * PAIR)), b = (float)(signed char)(x >> (16 * PAIR + 8));
@@ -171,5 +157,434 @@ template <int CODE, typename T, int PAIR> __device__ __forceinline__ unsigned wi
         }
     }
 }
+template <int CODE> __device__ __forceinline__ bool has_nan4(unsigned x) {   // e4m3 NaN: 0x7f or 0xff in a byte
+    return CODE == FLA_F8E4M3 && ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0);
+}
+
+// ---- one wave's walk over the keys ------------------------------------------------------------------------------
+// Where the 32 tokens of a step lie.  WIDE: pages hold at least 32 tokens, so a step has one page and everything about it
+// is uniform; else a lane knows the page of its eight tokens t0 + 8 g .. + 7.
+template <bool WIDE> struct Place {
+    int page;        // in the pool, whether held or not
+    bool held;       // false: nothing to see
+};
+
+// The table's entries for the next 64 (32 where a step has two pages) steps, one in each lane: a step reads its own with
+// no memory access, which would wait for every load issued before it.
+template <bool WIDE> struct PageWindow {
+    int entries;
+    __device__ __forceinline__ void fill(const AttnParams &p, const int32_t *row, int t0, int stride, int most) {
+        const int lane = threadIdx.x & 63;
+        const int64_t tok = WIDE ? (int64_t)t0 + (int64_t)lane * stride : (int64_t)t0 + (int64_t)(lane >> 1) * stride + 16 * (lane & 1);
+        const int64_t at = tok >> p.shift;
+        entries = tok < most && at < p.width ? row[at] : -1;      // a page behind the last token may be anything
+    }
+    __device__ __forceinline__ Place<WIDE> get(const AttnParams &p, const int32_t *row, int t0, int stride, int step, int most) {
+        if (step && (step & (WIDE ? 63 : 31)) == 0) fill(p, row, t0, stride, most);
+        const int k = step & (WIDE ? 63 : 31);
+        int page;
+        if (WIDE) page = __builtin_amdgcn_readlane(entries, k);
+        else {
+            const int a = __builtin_amdgcn_readlane(entries, 2 * k), b = __builtin_amdgcn_readlane(entries, 2 * k + 1);
+            page = (threadIdx.x & 32) ? b : a;
+        }
+        Place<WIDE> pl;
+        pl.held = (uint32_t)page < p.pool;
+        pl.page = pl.held ? page : 0;
+        return pl;
+    }
+};
+
+// lane offsets inside a page that hold for the whole walk (WIDE), in bytes
+struct LaneOffsets {
+    unsigned k, v;
+};
+
+template <int D, bool WIDE> struct KeyCodes {
+    u32x4 c[2][D / 64];
+    float scale;
+    __device__ __forceinline__ void load(const AttnParams &p, int head, int t0, const Place<WIDE> &pl, const LaneOffsets &off) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, in_page = (1 << p.shift) - 1;
+        scale = p.ks[(int64_t)pl.page * p.ks_p + head * p.ks_h];
+        const uint8_t *at;
+        if (WIDE) {
+            at = p.kc + (int64_t)pl.page * p.kc_p + (int64_t)head * p.kc_h + (int64_t)(t0 & in_page) * p.kc_t;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h) c[t][h] = *reinterpret_cast<const u32x4 *>(at + (off.k + (unsigned)(4 * t) * (unsigned)p.kc_t) + 64 * h);
+        } else {
+            // the rows of this lane are those of lane group i / 4, whose page sits in lane 16 (i / 4)
+            const int kg = i >> 2, page = __shfl(pl.page, kg * 16, kWave);
+            at = p.kc + (int64_t)page * p.kc_p + (int64_t)head * p.kc_h + (int64_t)(((t0 + 8 * kg) & in_page) + (i & 3)) * p.kc_t + g * 16;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h) c[t][h] = *reinterpret_cast<const u32x4 *>(at + 4 * t * p.kc_t + 64 * h);
+        }
+    }
+};
+
+template <int D, bool WIDE> struct ValueCodes {
+    unsigned c[8][D / 64];
+    float scale;
+    __device__ __forceinline__ void load(const AttnParams &p, int head, int t0, const Place<WIDE> &pl, const LaneOffsets &off) {
+        typedef unsigned VV __attribute__((ext_vector_type(D / 64)));
+        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, in_page = (1 << p.shift) - 1;
+        const float s = p.vs[(int64_t)pl.page * p.vs_p + head * p.vs_h];
+        scale = pl.held ? s : 0.f;
+        const uint8_t *at = p.vc + (int64_t)pl.page * p.vc_p + (int64_t)head * p.vc_h;
+        if (WIDE) at += (int64_t)(t0 & in_page) * p.vc_t;
+        else at += (int64_t)((t0 + 8 * g) & in_page) * p.vc_t + i * (D / 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint8_t *from = WIDE ? at + (off.v + (unsigned)e * (unsigned)p.vc_t) : at + e * p.vc_t;
+            if constexpr (D == 64) c[e][0] = *reinterpret_cast<const unsigned *>(from);
+            else {
+                const VV x = *reinterpret_cast<const VV *>(from);
+#pragma unroll
+                for (int w = 0; w < D / 64; ++w) c[e][w] = x[w];
+            }
+        }
+    }
+};
+
+// One wave: 16 NC query rows against the tokens it is led over, 32 at a time.
+//   S^T = K Q^T: tokens are the rows of the accumulators, query rows their columns; O^T += V^T P^T with P^T straight from
+//   the accumulator layout.
+//  - K: lane 16 g + i holds row i of a 16-token tile; it loads 16 bytes at 64 h + 16 g of its row, so a load touches whole
+//    64-byte pieces.  The contraction index is permuted by that; q is loaded with the same permutation.
+//  - rows are given to tokens so that the accumulators of lane group g are tokens 8 g .. 8 g + 7 of the step: the
+//    contraction order of O^T.  V: lane 16 g + i loads D/16 neighbouring channels of those eight tokens, and a byte
+//    transpose inside the lane gives the operands of D/16 tiles whose row i is channel D/16 i + j of tile j.
+//  - scales of pages multiply S after the product (exact codes enter the matrix unit) and P: the weight of a token is
+//    p vs / r with r the largest v scale so far (the accumulators are kept in units of r), rounded to fp16 with 11 bits:
+//    a bf16 weight would add an error as large as the rounding of the result.  vs / r enters as an addend of the
+//    exponent, which costs nothing for each element; pages whose scale is 0 or below r 2^-20 take a product instead.
+//  - the maximum moves only when a score passes it by 2^8 (weights then stay below 2^8, far inside fp16), so most steps
+//    need no exchange between lanes and no rescaling.
+// The next step's keys are loaded as soon as this step's are consumed, its values likewise.  Sums and statistics are fp32.
+template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
+    typedef typename Vec8<T>::type T8;
+    static constexpr float kMoveMax = 8.f, kFold = 0x1p-20f;
+    f32x4 o[NC][D / 16];   // o[c][j][e] of lane (g, i): channel D/16 (4 g + e) + j of query row 16 c + i, in units of r
+    float m[NC], l[NC];    // maximum in log2 (the same in all lanes of a column), this lane's share of the sum
+    float r;
+    u32x4 q[NC][D / 32];
+    int limit[NC];         // tokens that the column sees
+    int least, most;       // the smallest and largest limit of the wave's real columns
+
+    __device__ __forceinline__ void start(const AttnParams &p, const Request &rq, int head, int first_row) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+        const int cap = (int)min((int64_t)rq.len, (int64_t)p.width << p.shift);
+        least = INT32_MAX;
+        most = 0;
+        r = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int row = first_row + 16 * c + i, tok = row / p.group, h = head * p.group + row - tok * p.group;
+            const bool real = row < rq.rows;
+            limit[c] = real ? min(max(rq.len - rq.new_tokens + tok + 1, 0), cap) : 0;
+            const T *src = static_cast<const T *>(p.q) + (int64_t)(rq.first + (real ? tok : 0)) * p.q_t + (int64_t)(real ? h : 0) * p.q_h;
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) {
+                const u32x4 x = *reinterpret_cast<const u32x4 *>(src + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+                q[c][s] = real ? x : u32x4{0u, 0u, 0u, 0u};
+            }
+            int lo = real ? limit[c] : INT32_MAX, hi = limit[c];
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) {
+                lo = min(lo, __shfl_xor(lo, d, kWave));
+                hi = max(hi, __shfl_xor(hi, d, kWave));
+            }
+            least = min(least, lo);
+            most = max(most, hi);
+            m[c] = kNegInf;
+            l[c] = 0.f;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) o[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        least = __builtin_amdgcn_readfirstlane(least);
+        most = __builtin_amdgcn_readfirstlane(most);
+    }
+
+    // tokens t0, t0 + stride, ... (32 each) below end
+    __device__ __forceinline__ void run(const AttnParams &p, const int32_t *row, int head, int t0, int stride, int end) {
+        if (t0 >= end) return;
+        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+        LaneOffsets off;
+        off.k = (unsigned)(8 * (i >> 2) + (i & 3)) * (unsigned)p.kc_t + 16 * g;
+        off.v = (unsigned)(8 * g) * (unsigned)p.vc_t + i * (D / 16);
+        KeyCodes<D, WIDE> k;
+        ValueCodes<D, WIDE> v;
+        PageWindow<WIDE> pages;
+        pages.fill(p, row, t0, stride, most);
+        Place<WIDE> at = pages.get(p, row, t0, stride, 0, most);
+        k.load(p, head, t0, at, off);
+        v.load(p, head, t0, at, off);
+        for (int step = 1;; ++step) {
+            const int t1 = t0 + stride;
+            f32x4 s[NC][2];
+            scores(k, s);
+            const float f = k.scale * p.scale2;
+            Place<WIDE> next = at;
+            if (t1 < end) {
+                next = pages.get(p, row, t1, stride, step, most);
+                k.load(p, head, t1, next, off);
+            }
+            weigh(s, f, v, at.held, t0);
+            if (t1 >= end) break;
+            v.load(p, head, t1, next, off);
+            at = next;
+            t0 = t1;
+        }
+    }
+
+    __device__ __forceinline__ void scores(const KeyCodes<D, WIDE> &k, f32x4 (&s)[NC][2]) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const u32x4 a = {widen2<CODE, T, 0>(k.c[t][h][2 * half]), widen2<CODE, T, 1>(k.c[t][h][2 * half]),
+                                     widen2<CODE, T, 0>(k.c[t][h][2 * half + 1]), widen2<CODE, T, 1>(k.c[t][h][2 * half + 1])};
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+                        s[c][t] = mfma16x32(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, q[c][2 * h + half]), s[c][t]);
+                }
+    }
+
+    __device__ __forceinline__ void weigh(f32x4 (&s)[NC][2], float f, ValueCodes<D, WIDE> &v, bool held, int t0) {
+        const int tok = t0 + 8 * (int)((threadIdx.x & 63) >> 4);
+        const bool masked = t0 + 32 > least || __any(!held);      // some column does not see all of the step
+        bool nan = false;
+        if (masked) {
+            bool mine = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int x = 0; x < D / 64; ++x) {
+                    // tokens that no column sees must not enter the second product: 0 times a NaN is a NaN
+                    v.c[e][x] = tok + e < most && held ? v.c[e][x] : 0u;
+                    mine = mine || has_nan4<CODE>(v.c[e][x]);
+                }
+            nan = __any(mine);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[c][t][e] = tok + 4 * t + e < limit[c] && held ? s[c][t][e] * f : kNegInf;
+            f = 1.f;
+        }
+        bool move = false;
+        const bool negative = __any(f < 0.f);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float best = fmaxf(fmaxf(fmaxf(s[c][0][0], s[c][0][1]), fmaxf(s[c][0][2], s[c][0][3])), fmaxf(fmaxf(s[c][1][0], s[c][1][1]), fmaxf(s[c][1][2], s[c][1][3])));
+            if (negative && f < 0.f) best = fminf(fminf(fminf(s[c][0][0], s[c][0][1]), fminf(s[c][0][2], s[c][0][3])), fminf(fminf(s[c][1][0], s[c][1][1]), fminf(s[c][1][2], s[c][1][3])));
+            move = move || best * f > m[c] + kMoveMax;
+        }
+        if (__any(move)) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float best = m[c];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) best = fmaxf(best, s[c][t][e] * f);
+                best = fmaxf(best, __shfl_xor(best, 16, kWave));
+                best = fmaxf(best, __shfl_xor(best, 32, kWave));
+                const float by = best == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[c] - best);   // 0 before the first token
+                m[c] = best;
+                l[c] *= by;
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) o[c][j] *= by;
+            }
+        }
+        if (__any(v.scale > r)) {
+            float top = fmaxf(r, v.scale);
+            if (!WIDE) {
+                top = fmaxf(top, __shfl_xor(top, 16, kWave));
+                top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            }
+            const float by = r / top;
+            r = top;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) o[c][j] *= by;
+        }
+        f16x8 w[NC];
+        if (!__any(held && !(v.scale >= r * kFold && r > 0.f))) {
+            const float add = held ? __builtin_amdgcn_logf(v.scale / r) : 0.f, back = held ? r / v.scale : 1.f;   // log2
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float bias = add - (m[c] == kNegInf ? 0.f : m[c]);      // nothing seen yet: every weight is exp2(-inf) = 0
+                float sum = 0.f;
+                u32x4 packed;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[c][t][e], f, bias)), __builtin_amdgcn_exp2f(fmaf(s[c][t][e + 1], f, bias))};
+                        sum += x[0] + x[1];
+                        packed[2 * t + e / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, f16x2v));
+                    }
+                l[c] = fmaf(sum, back, l[c]);
+                w[c] = __builtin_bit_cast(f16x8, packed);
+            }
+        } else {
+            const float ratio = r > 0.f ? v.scale / r : 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float bias = m[c] == kNegInf ? 0.f : -m[c];
+                u32x4 packed;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[c][t][e], f, bias)), __builtin_amdgcn_exp2f(fmaf(s[c][t][e + 1], f, bias))};
+                        l[c] += x[0] + x[1];
+                        packed[2 * t + e / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(x * ratio, f16x2v));
+                    }
+                w[c] = __builtin_bit_cast(f16x8, packed);
+            }
+        }
+        if (nan) spread_nan(v, tok, held);
+        accumulate(v, w);
+    }
+
+    // A NaN in a token that some columns see and others do not: put into the columns that see it, taken out of the codes.
+    __device__ __forceinline__ void spread_nan(ValueCodes<D, WIDE> &v, int tok, bool held) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            u32x4 sees = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (tok + e < limit[c] && held) sees[e >> 1] |= (e & 1) ? 0x3c000000u : 0x00003c00u;
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    u32x4 bad = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (((v.c[e][x] >> (8 * j)) & 0x7fu) == 0x7fu) bad[e >> 1] |= (e & 1) ? 0x3c000000u : 0x00003c00u;
+                    const f32x4 hit = mfma16x32(__builtin_bit_cast(f16x8, bad), __builtin_bit_cast(f16x8, sees), f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (hit[e] > 0.f) o[c][4 * x + j][e] = __builtin_nanf("");
+                    __builtin_amdgcn_sched_barrier(0);                 // one at a time: this path must not cost registers
+                }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) {
+                unsigned is = (v.c[e][x] & 0x7f7f7f7fu) + 0x01010101u;   // 0x80 in the bytes that hold a NaN
+                is &= 0x80808080u;
+                v.c[e][x] &= ~((is << 1) - (is >> 7));
+            }
+    }
+
+    __device__ __forceinline__ void accumulate(const ValueCodes<D, WIDE> &v, const f16x8 (&w)[NC]) {   // O^T += V^T P^T
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) {
+            unsigned wide[8][2];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                wide[e][0] = widen2<CODE, f16, 0>(v.c[e][x]);
+                wide[e][1] = widen2<CODE, f16, 1>(v.c[e][x]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u32x4 a;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    a[e] = __builtin_amdgcn_perm(wide[2 * e + 1][j >> 1], wide[2 * e][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) o[c][4 * x + j] = mfma16x32(__builtin_bit_cast(f16x8, a), w[c], o[c][4 * x + j]);
+            }
+        }
+    }
+
+    // the sum over all lanes of each column; after the walk
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            l[c] += __shfl_xor(l[c], 16, kWave);
+            l[c] += __shfl_xor(l[c], 32, kWave);
+        }
+    }
+
+    // accumulators (already times r and joined with other waves', maximum mm, sum ll) to the result or the workspace
+    __device__ __forceinline__ void store(const AttnParams &p, const Request &rq, const Item &it, int64_t item, int head, int rows_per_tile,
+                                          int first_in_tile, const float (&mm)[NC], const float (&ll)[NC]) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int in_tile = first_in_tile + 16 * c + i, row = it.tile * rows_per_tile + in_tile;
+            if (row >= rq.rows) continue;
+            if (it.chunks == 1) {
+                const int tok = row / p.group, h = head * p.group + row - tok * p.group;
+                const float by = ll[c] > 0.f || ll[c] != ll[c] ? 1.f / ll[c] : 0.f;
+                T *dst = static_cast<T *>(p.out) + (int64_t)(rq.first + tok) * p.o_t + (int64_t)h * p.o_h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (D == 64) {
+                        typedef T T4 __attribute__((ext_vector_type(4)));
+                        T4 y;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[j] = (T)(o[c][j][e] * by);
+                        *reinterpret_cast<T4 *>(dst + 4 * (4 * g + e)) = y;
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < D / 128; ++x) {
+                            T8 y;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) y[j] = (T)(o[c][8 * x + j][e] * by);
+                            *reinterpret_cast<T8 *>(dst + D / 16 * (4 * g + e) + 8 * x) = y;
+                        }
+                    }
+                }
+                if (p.lse && g == 0) p.lse[(int64_t)(rq.first + tok) * p.lse_t + (int64_t)h * p.lse_h] = (mm[c] + log2f(ll[c])) * (1.f / kLog2e);
+            } else {
+                const int64_t slot = (item * p.heads + head) * rows_per_tile + in_tile;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int j = 0; j < D / 16; j += 4)
+                        *reinterpret_cast<f32x4 *>(p.part_o + slot * D + D / 16 * (4 * g + e) + j) = f32x4{o[c][j][e], o[c][j + 1][e], o[c][j + 2][e], o[c][j + 3][e]};
+                if (g == 0) {
+                    p.part_ml[slot * 2] = mm[c];
+                    p.part_ml[slot * 2 + 1] = ll[c];
+                }
+            }
+        }
+    }
+};
+
+// rows behind the last request: 0, lse -inf
+template <typename T, int THREADS> __device__ __forceinline__ void clear_tail(const AttnParams &p, int head, int D) {
+    const int from = min(max(p.cu[p.n], 0), p.tokens);
+    for (int64_t x = threadIdx.x; x < (int64_t)(p.tokens - from) * p.group * D; x += THREADS) {
+        const int64_t t = from + x / (p.group * D);
+        const int h = head * p.group + (int)(x / D % p.group), d = (int)(x % D);
+        static_cast<T *>(p.out)[t * p.o_t + h * p.o_h + d] = (T)0.f;
+        if (p.lse && d == 0) p.lse[t * p.lse_t + h * p.lse_h] = kNegInf;
+    }
+}
+
+struct AttnLaunch {
+    int nc, dim, code, dtype, longest_rows;
+    int64_t tiles, items;      // bounds
+    uint64_t o_bytes, bytes;
+};
+
+int launch_paged_prefill(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream);   // 64 (32 for D = 256) rows for a wave
 
 }  // namespace fla

@@ -1,0 +1,55 @@
+// paged_kv_attention for many query rows (chunked prefill): a wave takes 64 of them (32 for D = 256) over all their keys.
+// Bound by the vector and matrix units together.  For a 32-token step and D = 128 a wave issues 64 matrix instructions
+// (1024 clocks of the matrix pipe) and about 350 vector ones; codes are widened once for 64 rows, straight from the loads
+// of the wave, with no LDS and no barrier: the tiles of a head run on one XCD, whose L2 holds its keys.
+#include "paged_attention.h"
+
+namespace fla {
+namespace {
+
+template <typename T, int CODE, int D, int NC, bool WIDE>
+__global__ void __launch_bounds__(64) paged_prefill_kernel(const AttnParams p) {
+    constexpr int kRows = 16 * NC;
+    const int head = blockIdx.x % p.heads;
+    if (p.clear_tail && blockIdx.x < p.heads) clear_tail<T, 64>(p, head, D);
+    int base;
+    const int item = (gridDim.x - 1 - blockIdx.x) / p.heads;      // long rows of a request first
+    const Item it = find_item<kRows>(p, item, false, base);
+    if (!it.found) return;
+    const Request rq = request_of(p, it.r);
+    Walk<T, CODE, D, NC, WIDE> walk;
+    walk.start(p, rq, head, it.tile * kRows);
+    const int64_t from = (int64_t)it.chunk * it.units * kUnit;
+    const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
+    if (from < end) walk.run(p, p.table + it.r * p.table_s, head, (int)from, 32, end);
+    walk.finish();
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) walk.o[c][j] *= walk.r;
+    walk.store(p, rq, it, item, head, kRows, 0, walk.m, walk.l);
+}
+
+template <typename T, int CODE> int launch_dim(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
+    const dim3 grid((unsigned)(plan.items * p.heads));
+#define FLA_PREFILL(DD, NN)                                                                                                                     \
+    do {                                                                                                                                        \
+        if (p.shift >= 5) FLA_LAUNCH("paged_kv_attention", stream, (paged_prefill_kernel<T, CODE, DD, NN, true>), grid, dim3(64), 0, stream, p);  \
+        else FLA_LAUNCH("paged_kv_attention", stream, (paged_prefill_kernel<T, CODE, DD, NN, false>), grid, dim3(64), 0, stream, p);              \
+    } while (0)
+    if (plan.dim == 64) FLA_PREFILL(64, 4);
+    else if (plan.dim == 128) FLA_PREFILL(128, 4);
+    else FLA_PREFILL(256, 2);
+#undef FLA_PREFILL
+    FLA_HIP_CHECK(hipGetLastError());
+    return FLA_OK;
+}
+
+}  // namespace
+
+int launch_paged_prefill(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
+    if (plan.dtype == FLA_BF16) return plan.code == FLA_I8 ? launch_dim<bf16, FLA_I8>(p, plan, stream) : launch_dim<bf16, FLA_F8E4M3>(p, plan, stream);
+    return plan.code == FLA_I8 ? launch_dim<f16, FLA_I8>(p, plan, stream) : launch_dim<f16, FLA_F8E4M3>(p, plan, stream);
+}
+
+}  // namespace fla
