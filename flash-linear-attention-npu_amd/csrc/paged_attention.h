@@ -173,20 +173,20 @@ template <bool WIDE> struct Place {
 // no memory access, which would wait for every load issued before it.
 template <bool WIDE> struct PageWindow {
     int entries;
-    __device__ __forceinline__ void fill(const AttnParams &p, const int32_t *row, int t0, int stride, int most) {
+    __device__ __forceinline__ void fill(const AttnParams &p, const int32_t *row, int t0, int stride) {
         const int lane = threadIdx.x & 63;
         const int64_t tok = WIDE ? (int64_t)t0 + (int64_t)lane * stride : (int64_t)t0 + (int64_t)(lane >> 1) * stride + 16 * (lane & 1);
         const int64_t at = tok >> p.shift;
-        entries = tok < most && at < p.width ? row[at] : -1;      // a page behind the last token may be anything
+        entries = at < p.width ? row[at] : -1;
     }
     __device__ __forceinline__ Place<WIDE> get(const AttnParams &p, const int32_t *row, int t0, int stride, int step, int most) {
-        if (step && (step & (WIDE ? 63 : 31)) == 0) fill(p, row, t0, stride, most);
+        if (step && (step & (WIDE ? 63 : 31)) == 0) fill(p, row, t0, stride);
         const int k = step & (WIDE ? 63 : 31);
         int page;
         if (WIDE) page = __builtin_amdgcn_readlane(entries, k);
-        else {
+        else {                            // a page behind the last token may be anything
             const int a = __builtin_amdgcn_readlane(entries, 2 * k), b = __builtin_amdgcn_readlane(entries, 2 * k + 1);
-            page = (threadIdx.x & 32) ? b : a;
+            page = !(threadIdx.x & 32) ? a : t0 + 16 < most ? b : -1;
         }
         Place<WIDE> pl;
         pl.held = (uint32_t)page < p.pool;
@@ -200,7 +200,13 @@ struct LaneOffsets {
     unsigned k, v;
 };
 
-template <int D, bool WIDE> struct KeyCodes {
+// STREAM: loads that do not stay in the caches.
+template <bool STREAM, typename V> __device__ __forceinline__ V load_codes(const uint8_t *p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
+    else return *reinterpret_cast<const V *>(p);
+}
+
+template <int D, bool WIDE, bool STREAM> struct KeyCodes {
     u32x4 c[2][D / 64];
     float scale;
     __device__ __forceinline__ void load(const AttnParams &p, int head, int t0, const Place<WIDE> &pl, const LaneOffsets &off) {
@@ -212,7 +218,7 @@ template <int D, bool WIDE> struct KeyCodes {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) c[t][h] = *reinterpret_cast<const u32x4 *>(at + (off.k + (unsigned)(4 * t) * (unsigned)p.kc_t) + 64 * h);
+                for (int h = 0; h < D / 64; ++h) c[t][h] = load_codes<STREAM, u32x4>(at + (off.k + (unsigned)(4 * t) * (unsigned)p.kc_t) + 64 * h);
         } else {
             // the rows of this lane are those of lane group i / 4, whose page sits in lane 16 (i / 4)
             const int kg = i >> 2, page = __shfl(pl.page, kg * 16, kWave);
@@ -220,12 +226,12 @@ template <int D, bool WIDE> struct KeyCodes {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) c[t][h] = *reinterpret_cast<const u32x4 *>(at + 4 * t * p.kc_t + 64 * h);
+                for (int h = 0; h < D / 64; ++h) c[t][h] = load_codes<STREAM, u32x4>(at + 4 * t * p.kc_t + 64 * h);
         }
     }
 };
 
-template <int D, bool WIDE> struct ValueCodes {
+template <int D, bool WIDE, bool STREAM> struct ValueCodes {
     unsigned c[8][D / 64];
     float scale;
     __device__ __forceinline__ void load(const AttnParams &p, int head, int t0, const Place<WIDE> &pl, const LaneOffsets &off) {
@@ -239,9 +245,9 @@ template <int D, bool WIDE> struct ValueCodes {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint8_t *from = WIDE ? at + (off.v + (unsigned)e * (unsigned)p.vc_t) : at + e * p.vc_t;
-            if constexpr (D == 64) c[e][0] = *reinterpret_cast<const unsigned *>(from);
+            if constexpr (D == 64) c[e][0] = load_codes<STREAM, unsigned>(from);
             else {
-                const VV x = *reinterpret_cast<const VV *>(from);
+                const VV x = load_codes<STREAM, VV>(from);
 #pragma unroll
                 for (int w = 0; w < D / 64; ++w) c[e][w] = x[w];
             }
@@ -264,8 +270,8 @@ template <int D, bool WIDE> struct ValueCodes {
 //  - the maximum moves only when a score passes it by 2^8 (weights then stay below 2^8, far inside fp16), so most steps
 //    need no exchange between lanes and no rescaling.
 // The next step's keys are loaded as soon as this step's are consumed, its values likewise.  Sums and statistics are fp32.
-template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
-    typedef typename Vec8<T>::type T8;
+template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
+    typedef elemx8 T8;
     static constexpr float kMoveMax = 8.f, kFold = 0x1p-20f;
     f32x4 o[NC][D / 16];   // o[c][j][e] of lane (g, i): channel D/16 (4 g + e) + j of query row 16 c + i, in units of r
     float m[NC], l[NC];    // maximum in log2 (the same in all lanes of a column), this lane's share of the sum
@@ -285,7 +291,7 @@ template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
             const int row = first_row + 16 * c + i, tok = row / p.group, h = head * p.group + row - tok * p.group;
             const bool real = row < rq.rows;
             limit[c] = real ? min(max(rq.len - rq.new_tokens + tok + 1, 0), cap) : 0;
-            const T *src = static_cast<const T *>(p.q) + (int64_t)(rq.first + (real ? tok : 0)) * p.q_t + (int64_t)(real ? h : 0) * p.q_h;
+            const elem *src = static_cast<const elem *>(p.q) + (int64_t)(rq.first + (real ? tok : 0)) * p.q_t + (int64_t)(real ? h : 0) * p.q_h;
 #pragma unroll
             for (int s = 0; s < D / 32; ++s) {
                 const u32x4 x = *reinterpret_cast<const u32x4 *>(src + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
@@ -308,17 +314,15 @@ template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
         most = __builtin_amdgcn_readfirstlane(most);
     }
 
-    // tokens t0, t0 + stride, ... (32 each) below end
-    __device__ __forceinline__ void run(const AttnParams &p, const int32_t *row, int head, int t0, int stride, int end) {
+    // tokens t0, t0 + stride, ... (32 each) below end <= most; pages: filled for t0 (before start, which waits for lengths)
+    __device__ __forceinline__ void run(const AttnParams &p, const int32_t *row, PageWindow<WIDE> &pages, int head, int t0, int stride, int end) {
         if (t0 >= end) return;
         const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
         LaneOffsets off;
         off.k = (unsigned)(8 * (i >> 2) + (i & 3)) * (unsigned)p.kc_t + 16 * g;
         off.v = (unsigned)(8 * g) * (unsigned)p.vc_t + i * (D / 16);
-        KeyCodes<D, WIDE> k;
-        ValueCodes<D, WIDE> v;
-        PageWindow<WIDE> pages;
-        pages.fill(p, row, t0, stride, most);
+        KeyCodes<D, WIDE, STREAM> k;
+        ValueCodes<D, WIDE, STREAM> v;
         Place<WIDE> at = pages.get(p, row, t0, stride, 0, most);
         k.load(p, head, t0, at, off);
         v.load(p, head, t0, at, off);
@@ -340,7 +344,7 @@ template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
         }
     }
 
-    __device__ __forceinline__ void scores(const KeyCodes<D, WIDE> &k, f32x4 (&s)[NC][2]) {
+    __device__ __forceinline__ void scores(const KeyCodes<D, WIDE, STREAM> &k, f32x4 (&s)[NC][2]) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -349,15 +353,15 @@ template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const u32x4 a = {widen2<CODE, T, 0>(k.c[t][h][2 * half]), widen2<CODE, T, 1>(k.c[t][h][2 * half]),
-                                     widen2<CODE, T, 0>(k.c[t][h][2 * half + 1]), widen2<CODE, T, 1>(k.c[t][h][2 * half + 1])};
+                    const u32x4 a = {widen2<CODE, elem, 0>(k.c[t][h][2 * half]), widen2<CODE, elem, 1>(k.c[t][h][2 * half]),
+                                     widen2<CODE, elem, 0>(k.c[t][h][2 * half + 1]), widen2<CODE, elem, 1>(k.c[t][h][2 * half + 1])};
 #pragma unroll
                     for (int c = 0; c < NC; ++c)
                         s[c][t] = mfma16x32(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, q[c][2 * h + half]), s[c][t]);
                 }
     }
 
-    __device__ __forceinline__ void weigh(f32x4 (&s)[NC][2], float f, ValueCodes<D, WIDE> &v, bool held, int t0) {
+    __device__ __forceinline__ void weigh(f32x4 (&s)[NC][2], float f, ValueCodes<D, WIDE, STREAM> &v, bool held, int t0) {
         const int tok = t0 + 8 * (int)((threadIdx.x & 63) >> 4);
         const bool masked = t0 + 32 > least || __any(!held);      // some column does not see all of the step
         bool nan = false;
@@ -459,7 +463,7 @@ template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
     }
 
     // A NaN in a token that some columns see and others do not: put into the columns that see it, taken out of the codes.
-    __device__ __forceinline__ void spread_nan(ValueCodes<D, WIDE> &v, int tok, bool held) {
+    __device__ __forceinline__ void spread_nan(ValueCodes<D, WIDE, STREAM> &v, int tok, bool held) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             u32x4 sees = {0u, 0u, 0u, 0u};
@@ -491,7 +495,7 @@ template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
             }
     }
 
-    __device__ __forceinline__ void accumulate(const ValueCodes<D, WIDE> &v, const f16x8 (&w)[NC]) {   // O^T += V^T P^T
+    __device__ __forceinline__ void accumulate(const ValueCodes<D, WIDE, STREAM> &v, const f16x8 (&w)[NC]) {   // O^T += V^T P^T
 #pragma unroll
         for (int x = 0; x < D / 64; ++x) {
             unsigned wide[8][2];
@@ -532,21 +536,20 @@ template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
             if (it.chunks == 1) {
                 const int tok = row / p.group, h = head * p.group + row - tok * p.group;
                 const float by = ll[c] > 0.f || ll[c] != ll[c] ? 1.f / ll[c] : 0.f;
-                T *dst = static_cast<T *>(p.out) + (int64_t)(rq.first + tok) * p.o_t + (int64_t)h * p.o_h;
+                elem *dst = static_cast<elem *>(p.out) + (int64_t)(rq.first + tok) * p.o_t + (int64_t)h * p.o_h;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (D == 64) {
-                        typedef T T4 __attribute__((ext_vector_type(4)));
-                        T4 y;
+                        elemx4 y;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) y[j] = (T)(o[c][j][e] * by);
-                        *reinterpret_cast<T4 *>(dst + 4 * (4 * g + e)) = y;
+                        for (int j = 0; j < 4; ++j) y[j] = (elem)(o[c][j][e] * by);
+                        *reinterpret_cast<elemx4 *>(dst + 4 * (4 * g + e)) = y;
                     } else {
 #pragma unroll
                         for (int x = 0; x < D / 128; ++x) {
                             T8 y;
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) y[j] = (T)(o[c][8 * x + j][e] * by);
+                            for (int j = 0; j < 8; ++j) y[j] = (elem)(o[c][8 * x + j][e] * by);
                             *reinterpret_cast<T8 *>(dst + D / 16 * (4 * g + e) + 8 * x) = y;
                         }
                     }
@@ -569,22 +572,33 @@ template <typename T, int CODE, int D, int NC, bool WIDE> struct Walk {
 };
 
 // rows behind the last request: 0, lse -inf
-template <typename T, int THREADS> __device__ __forceinline__ void clear_tail(const AttnParams &p, int head, int D) {
+template <int THREADS> __device__ __forceinline__ void clear_tail(const AttnParams &p, int head, int D) {
     const int from = min(max(p.cu[p.n], 0), p.tokens);
     for (int64_t x = threadIdx.x; x < (int64_t)(p.tokens - from) * p.group * D; x += THREADS) {
         const int64_t t = from + x / (p.group * D);
         const int h = head * p.group + (int)(x / D % p.group), d = (int)(x % D);
-        static_cast<T *>(p.out)[t * p.o_t + h * p.o_h + d] = (T)0.f;
+        static_cast<elem *>(p.out)[t * p.o_t + h * p.o_h + d] = (elem)0.f;
         if (p.lse && d == 0) p.lse[t * p.lse_t + h * p.lse_h] = kNegInf;
     }
 }
 
 struct AttnLaunch {
-    int nc, dim, code, dtype, longest_rows;
+    int nc, dim, code, waves, longest_rows;
     int64_t tiles, items;      // bounds
     uint64_t o_bytes, bytes;
 };
 
-int launch_paged_prefill(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream);   // 64 (32 for D = 256) rows for a wave
+// The kernels are built once for each query type (the bf16 and the f16 object of their sources).
+int launch_paged_decode(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream);
+int launch_paged_decode_f16(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream);
+int launch_paged_prefill(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream);
+int launch_paged_prefill_f16(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream);
+int launch_paged_join(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream);
+int launch_paged_join_f16(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream);
+#ifdef FLA_ELEM_F16
+#define FLA_PAGED(name) name##_f16
+#else
+#define FLA_PAGED(name) name
+#endif
 
 }  // namespace fla

@@ -1,187 +1,8 @@
-// paged_kv_attention: softmax attention of a few query rows over a paged cache held in 8 bits (decode, checking of
-// speculated tokens), the join of split key axes, and the entry point.
-//   s_t = scale * ks_page (q . k8_t),  o = sum_t e^{s_t - m} vs_page v8_t / sum_t e^{s_t - m}
-// Bound by HBM: each code is read once.  The waves of a workgroup take 32-token steps of a chunk in turn, each with its own
-// running maximum, sum and accumulators (the walk of paged_attention.h: no LDS, no barrier), and are joined once at the end.
+// Entry point of paged_kv_attention: checks, the choice of kernel and split, and the launches.
 #include "paged_attention.h"
 
 namespace fla {
 namespace {
-
-template <typename T, int CODE, int D, int NC, int W, bool WIDE>
-__global__ void __launch_bounds__(W * 64) paged_decode_kernel(const AttnParams p) {
-    constexpr int kRows = 16 * NC;
-    __shared__ float lds_ml[W][kRows][2];
-    extern __shared__ float lds_o[];                       // [W/2][kRows][D]
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i = lane & 15;
-    const int head = blockIdx.x % p.heads, item = blockIdx.x / p.heads;
-    if (p.clear_tail && blockIdx.x >= gridDim.x - p.heads) clear_tail<T, W * 64>(p, head, D);
-    int base;
-    const Item it = find_item<kRows>(p, item, false, base);
-    if (!it.found) return;
-    const Request rq = request_of(p, it.r);
-    Walk<T, CODE, D, NC, WIDE> walk;
-    walk.start(p, rq, head, it.tile * kRows);
-    const int64_t from = (int64_t)it.chunk * it.units * kUnit;
-    const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
-    if (from < end) walk.run(p, p.table + it.r * p.table_s, head, (int)from + 32 * wave, 32 * W, end);
-    walk.finish();
-    // join the waves: statistics first, then the accumulators pairwise through LDS
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-        if (g == 0) {
-            lds_ml[wave][16 * c + i][0] = walk.m[c];
-            lds_ml[wave][16 * c + i][1] = walk.l[c];
-        }
-    __syncthreads();
-    float m[NC], l[NC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        m[c] = kNegInf;
-        l[c] = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) m[c] = fmaxf(m[c], lds_ml[w][16 * c + i][0]);
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float lw = lds_ml[w][16 * c + i][1];      // 0: the wave saw no token (its maximum is -inf)
-            l[c] += lw == 0.f ? 0.f : lw * exp2f(lds_ml[w][16 * c + i][0] - m[c]);
-        }
-        const float by = walk.l[c] == 0.f ? 0.f : exp2f(walk.m[c] - m[c]) * walk.r;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) walk.o[c][j] *= by;
-    }
-#pragma unroll
-    for (int half = W / 2; half >= 1; half >>= 1) {
-        if (wave >= half && wave < 2 * half) {
-            f32x4 *dst = reinterpret_cast<f32x4 *>(lds_o + (size_t)(wave - half) * kRows * D);
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) dst[(c * (D / 16) + j) * 64 + lane] = walk.o[c][j];
-        }
-        __syncthreads();
-        if (wave < half) {
-            const f32x4 *src = reinterpret_cast<const f32x4 *>(lds_o + (size_t)wave * kRows * D);
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) walk.o[c][j] += src[(c * (D / 16) + j) * 64 + lane];
-        }
-        if (half > 1) __syncthreads();
-    }
-    if (wave == 0) walk.store(p, rq, it, item, head, kRows, 0, m, l);
-}
-
-// Joins the chunks of a tile: one workgroup for each (tile, cache head, query row), whose waves take the chunks in turn.
-constexpr int kJoinWaves = 4;
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(64 * kJoinWaves) paged_join_kernel(const AttnParams p) {
-    constexpr int V = D / 64;
-    __shared__ float lds_m[kJoinWaves], lds_l[kJoinWaves], lds_o[kJoinWaves][D];
-    int base;
-    const int head = blockIdx.x % p.heads;
-    const Item it = find_item<ROWS>(p, blockIdx.x / p.heads, true, base);
-    if (!it.found || it.chunks == 1) return;
-    const Request rq = request_of(p, it.r);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = min(ROWS, rq.rows - it.tile * ROWS);
-    for (int in_tile = blockIdx.y; in_tile < rows; in_tile += gridDim.y) {
-        const int r = it.tile * ROWS + in_tile;
-        const int64_t first = ((int64_t)base * p.heads + head) * ROWS + in_tile, step = (int64_t)p.heads * ROWS;
-        float m = kNegInf, l = 0.f, o[V];
-#pragma unroll
-        for (int x = 0; x < V; ++x) o[x] = 0.f;
-        for (int c0 = wave; c0 < it.chunks; c0 += 4 * kJoinWaves) {      // four chunks in flight
-            float mc[4], lc[4], oc[4][V], best = m;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int c = c0 + u * kJoinWaves;
-                const int64_t slot = first + min(c, it.chunks - 1) * step;
-                mc[u] = p.part_ml[slot * 2];
-                lc[u] = c < it.chunks ? p.part_ml[slot * 2 + 1] : 0.f;
-#pragma unroll
-                for (int x = 0; x < V; ++x) oc[u][x] = p.part_o[slot * D + lane * V + x];
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) best = fmaxf(best, mc[u]);
-            const float old = l == 0.f ? 0.f : exp2f(m - best);
-            l *= old;
-#pragma unroll
-            for (int x = 0; x < V; ++x) o[x] *= old;
-            m = best;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float by = lc[u] == 0.f ? 0.f : exp2f(mc[u] - best);        // a sum of 0: the chunk has no token that the row sees
-                l += by * lc[u];
-#pragma unroll
-                for (int x = 0; x < V; ++x) o[x] += lc[u] == 0.f ? 0.f : by * oc[u][x];
-            }
-        }
-        if (lane == 0) {
-            lds_m[wave] = m;
-            lds_l[wave] = l;
-        }
-#pragma unroll
-        for (int x = 0; x < V; ++x) lds_o[wave][lane * V + x] = o[x];
-        __syncthreads();
-        if (wave == 0) {
-            float best = kNegInf, sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < kJoinWaves; ++w) best = fmaxf(best, lds_m[w]);
-#pragma unroll
-            for (int x = 0; x < V; ++x) o[x] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kJoinWaves; ++w) {
-                const float lw = lds_l[w], by = lw == 0.f ? 0.f : exp2f(lds_m[w] - best);
-                sum += by * lw;
-#pragma unroll
-                for (int x = 0; x < V; ++x) o[x] += lw == 0.f ? 0.f : by * lds_o[w][lane * V + x];
-            }
-            const int tok = r / p.group, h = head * p.group + r - tok * p.group;
-            const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-            T *dst = static_cast<T *>(p.out) + (int64_t)(rq.first + tok) * p.o_t + (int64_t)h * p.o_h;
-#pragma unroll
-            for (int x = 0; x < V; ++x) dst[lane * V + x] = (T)(o[x] * by);
-            if (p.lse && lane == 0) p.lse[(int64_t)(rq.first + tok) * p.lse_t + (int64_t)h * p.lse_h] = (best + log2f(sum)) * (1.f / kLog2e);
-        }
-        __syncthreads();
-    }
-}
-
-template <typename T, int CODE, int D, int NC, bool WIDE> int launch_decode(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
-    constexpr int W = NC * D <= 128 ? 8 : 4;
-    const dim3 grid((unsigned)(plan.items * p.heads));
-    const size_t lds = (size_t)(W / 2) * 16 * NC * D * 4;
-    const auto kernel = paged_decode_kernel<T, CODE, D, NC, W, WIDE>;
-    if (lds > 48 * 1024) FLA_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    FLA_LAUNCH("paged_kv_attention", stream, kernel, grid, dim3(W * 64), lds, stream, p);
-    FLA_HIP_CHECK(hipGetLastError());
-    return FLA_OK;
-}
-
-template <typename T, int ROWS> int launch_join(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
-    const dim3 grid((unsigned)(plan.tiles * p.heads), (unsigned)(plan.longest_rows < ROWS ? plan.longest_rows : ROWS)), block(64 * kJoinWaves);
-    if (plan.dim == 64) FLA_LAUNCH("paged_kv_attention_join", stream, (paged_join_kernel<T, 64, ROWS>), grid, block, 0, stream, p);
-    else if (plan.dim == 128) FLA_LAUNCH("paged_kv_attention_join", stream, (paged_join_kernel<T, 128, ROWS>), grid, block, 0, stream, p);
-    else FLA_LAUNCH("paged_kv_attention_join", stream, (paged_join_kernel<T, 256, ROWS>), grid, block, 0, stream, p);
-    FLA_HIP_CHECK(hipGetLastError());
-    return FLA_OK;
-}
-
-template <typename T, int CODE> int launch_dim(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
-    const bool wide = p.shift >= 5;
-#define FLA_NC(DD, NN) return wide ? launch_decode<T, CODE, DD, NN, true>(p, plan, stream) : launch_decode<T, CODE, DD, NN, false>(p, plan, stream)
-    if (plan.dim == 64) {
-        if (plan.nc == 1) FLA_NC(64, 1);
-        FLA_NC(64, 2);
-    } else if (plan.dim == 128) {
-        if (plan.nc == 1) FLA_NC(128, 1);
-        FLA_NC(128, 2);
-    } else {
-        if (plan.nc == 1) FLA_NC(256, 1);
-        FLA_NC(256, 2);
-    }
-#undef FLA_NC
-}
 
 inline bool present(const fla_tensor *t) { return t != nullptr && t->data != nullptr; }
 
@@ -232,18 +53,30 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
     AttnParams p{};
     const int64_t longest = !present(cu) ? 1 : max_query_len ? (max_query_len < T ? max_query_len : T) : T;
     plan.longest_rows = (int)(longest * group < 4096 ? longest * group : 4096);
-    const bool prefill = longest * group > 32;
-    plan.nc = prefill ? (dim == 256 ? 2 : 4) : longest * group > 16 ? 2 : 1;
+    // Up to 64 rows (32 for D = 256, whose accumulators take twice the registers) go to the kernel whose waves share a tile.
+    const int64_t rows_most = longest * group, tile_most = dim == 256 ? 32 : 64;
+    const bool prefill = rows_most > tile_most;
+    plan.nc = rows_most <= 16 ? 1 : rows_most <= 32 || dim == 256 ? 2 : 4;
     plan.dim = (int)dim;
     plan.code = shape.code;
-    plan.dtype = q->dtype;
     const int64_t rows = 16 * plan.nc;
     plan.tiles = present(cu) ? T * group / rows + n : n * ((group + rows - 1) / rows);
     p.tiles_each = (int)((group + rows - 1) / rows);
-    p.target = (int)((1024 + shape.heads - 1) / shape.heads);
-    p.min_units = 8;
-    const int64_t capacity = table->shape[1] << shape.shift;
-    if (prefill ? plan.tiles * shape.heads >= 1024 : capacity <= 2048) p.target = 0;
+    // The split of the key axis.  Lengths are on the device; the host knows the most that a row of the table can name.
+    //  - decode: chunks of at least 256 tokens; about 512 workgroups where there are few tiles, 2048 where tiles alone fill
+    //    the chip, since ragged requests balance better (32 heads on 8 of 128, e4m3: one request of 262 k tokens 102 us with
+    //    512 and 115 us with 2048 workgroups; 128 requests of up to 8 k 239 and 211 us);
+    //  - tables of at most 2048 tokens: one chunk and one launch, of eight waves (four requests of 1100: 11.8 us against 12 us
+    //    with two launches on the GPU, and one launch less on the host);
+    //  - prefill: only where tiles would leave compute units idle.
+    const int64_t capacity = table->shape[1] << shape.shift, tiles_all = plan.tiles * shape.heads;
+    plan.waves = 4;
+    p.min_units = 4;
+    p.target = (int)(((prefill ? 1024 : tiles_all < 256 ? 512 : 2048) + shape.heads - 1) / shape.heads);
+    if (prefill ? tiles_all >= 1024 : capacity <= 2048) {
+        p.target = 0;
+        if (plan.nc == 1 && tiles_all < 512) plan.waves = 8;
+    }
     plan.items = plan.tiles + p.target;
     FLA_REQUIRE(capacity <= INT32_MAX - 65536, FLA_ERR_SHAPE, "%s: a row of block_table names more than 2^31 - 2^16 tokens.", op);
     FLA_REQUIRE(plan.items * shape.heads < ((int64_t)1 << 31), FLA_ERR_SHAPE, "%s: too many query rows.", op);
@@ -294,13 +127,11 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
     p.pool = (uint32_t)shape.pool;
     p.scale2 = (float)(scale * 1.44269504088896340736);
     p.clear_tail = clear_tail && p.cu;
-    if (prefill) rc = launch_paged_prefill(p, plan, stream);
-    else if (q->dtype == FLA_BF16) rc = shape.code == FLA_I8 ? launch_dim<bf16, FLA_I8>(p, plan, stream) : launch_dim<bf16, FLA_F8E4M3>(p, plan, stream);
-    else rc = shape.code == FLA_I8 ? launch_dim<f16, FLA_I8>(p, plan, stream) : launch_dim<f16, FLA_F8E4M3>(p, plan, stream);
+    const bool f16_rows = q->dtype == FLA_F16;
+    if (prefill) rc = f16_rows ? launch_paged_prefill_f16(p, plan, stream) : launch_paged_prefill(p, plan, stream);
+    else rc = f16_rows ? launch_paged_decode_f16(p, plan, stream) : launch_paged_decode(p, plan, stream);
     if (rc || !p.target) return rc;
-#define FLA_JOIN(T) (plan.nc == 1 ? launch_join<T, 16>(p, plan, stream) : plan.nc == 2 ? launch_join<T, 32>(p, plan, stream) : launch_join<T, 64>(p, plan, stream))
-    return q->dtype == FLA_BF16 ? FLA_JOIN(bf16) : FLA_JOIN(f16);
-#undef FLA_JOIN
+    return f16_rows ? launch_paged_join_f16(p, plan, stream) : launch_paged_join(p, plan, stream);
 }
 
 }  // namespace

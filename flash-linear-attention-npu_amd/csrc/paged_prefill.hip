@@ -7,21 +7,25 @@
 namespace fla {
 namespace {
 
-template <typename T, int CODE, int D, int NC, bool WIDE>
+template <int CODE, int D, int NC, bool WIDE>
 __global__ void __launch_bounds__(64) paged_prefill_kernel(const AttnParams p) {
     constexpr int kRows = 16 * NC;
     const int head = blockIdx.x % p.heads;
-    if (p.clear_tail && blockIdx.x < p.heads) clear_tail<T, 64>(p, head, D);
+    if (p.clear_tail && blockIdx.x < p.heads) clear_tail<64>(p, head, D);
     int base;
     const int item = (gridDim.x - 1 - blockIdx.x) / p.heads;      // long rows of a request first
     const Item it = find_item<kRows>(p, item, false, base);
     if (!it.found) return;
-    const Request rq = request_of(p, it.r);
-    Walk<T, CODE, D, NC, WIDE> walk;
-    walk.start(p, rq, head, it.tile * kRows);
     const int64_t from = (int64_t)it.chunk * it.units * kUnit;
+    const int t0 = (int)min(from, (int64_t)INT32_MAX - 65536);
+    const int32_t *row = p.table + it.r * p.table_s;
+    PageWindow<WIDE> pages;
+    pages.fill(p, row, t0, 32);
+    const Request rq = request_of(p, it.r);
+    Walk<CODE, D, NC, WIDE, false> walk;
+    walk.start(p, rq, head, it.tile * kRows);
     const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
-    if (from < end) walk.run(p, p.table + it.r * p.table_s, head, (int)from, 32, end);
+    walk.run(p, row, pages, head, t0, 32, end);
     walk.finish();
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -30,12 +34,12 @@ __global__ void __launch_bounds__(64) paged_prefill_kernel(const AttnParams p) {
     walk.store(p, rq, it, item, head, kRows, 0, walk.m, walk.l);
 }
 
-template <typename T, int CODE> int launch_dim(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
+template <int CODE> int launch_dim(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
     const dim3 grid((unsigned)(plan.items * p.heads));
 #define FLA_PREFILL(DD, NN)                                                                                                                     \
     do {                                                                                                                                        \
-        if (p.shift >= 5) FLA_LAUNCH("paged_kv_attention", stream, (paged_prefill_kernel<T, CODE, DD, NN, true>), grid, dim3(64), 0, stream, p);  \
-        else FLA_LAUNCH("paged_kv_attention", stream, (paged_prefill_kernel<T, CODE, DD, NN, false>), grid, dim3(64), 0, stream, p);              \
+        if (p.shift >= 5) FLA_LAUNCH("paged_kv_attention", stream, (paged_prefill_kernel<CODE, DD, NN, true>), grid, dim3(64), 0, stream, p);  \
+        else FLA_LAUNCH("paged_kv_attention", stream, (paged_prefill_kernel<CODE, DD, NN, false>), grid, dim3(64), 0, stream, p);              \
     } while (0)
     if (plan.dim == 64) FLA_PREFILL(64, 4);
     else if (plan.dim == 128) FLA_PREFILL(128, 4);
@@ -47,9 +51,8 @@ template <typename T, int CODE> int launch_dim(const AttnParams &p, const AttnLa
 
 }  // namespace
 
-int launch_paged_prefill(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
-    if (plan.dtype == FLA_BF16) return plan.code == FLA_I8 ? launch_dim<bf16, FLA_I8>(p, plan, stream) : launch_dim<bf16, FLA_F8E4M3>(p, plan, stream);
-    return plan.code == FLA_I8 ? launch_dim<f16, FLA_I8>(p, plan, stream) : launch_dim<f16, FLA_F8E4M3>(p, plan, stream);
+int FLA_PAGED(launch_paged_prefill)(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
+    return plan.code == FLA_I8 ? launch_dim<FLA_I8>(p, plan, stream) : launch_dim<FLA_F8E4M3>(p, plan, stream);
 }
 
 }  // namespace fla
