@@ -218,7 +218,7 @@ template <int D, bool WIDE, bool STREAM> struct KeyCodes {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) c[t][h] = load_codes<STREAM, u32x4>(at + (off.k + (unsigned)(4 * t) * (unsigned)p.kc_t) + 64 * h);
+                for (int h = 0; h < D / 64; ++h) c[t][h] = load_codes<STREAM, u32x4>(at + (int64_t)(4 * t) * p.kc_t + 64 * h + off.k);
         } else {
             // the rows of this lane are those of lane group i / 4, whose page sits in lane 16 (i / 4)
             const int kg = i >> 2, page = __shfl(pl.page, kg * 16, kWave);
@@ -244,7 +244,7 @@ template <int D, bool WIDE, bool STREAM> struct ValueCodes {
         else at += (int64_t)((t0 + 8 * g) & in_page) * p.vc_t + i * (D / 16);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint8_t *from = WIDE ? at + (off.v + (unsigned)e * (unsigned)p.vc_t) : at + e * p.vc_t;
+            const uint8_t *from = WIDE ? at + (int64_t)e * p.vc_t + off.v : at + e * p.vc_t;
             if constexpr (D == 64) c[e][0] = load_codes<STREAM, unsigned>(from);
             else {
                 const VV x = load_codes<STREAM, VV>(from);
@@ -276,11 +276,14 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
     f32x4 o[NC][D / 16];   // o[c][j][e] of lane (g, i): channel D/16 (4 g + e) + j of query row 16 c + i, in units of r
     float m[NC], l[NC];    // maximum in log2 (the same in all lanes of a column), this lane's share of the sum
     float r;
-    u32x4 q[NC][D / 32];
+    static constexpr bool kQueriesInLds = NC > 1;
+    u32x4 q[kQueriesInLds ? 1 : NC][D / 32];
+    u32x4 *lds_q;          // [NC][D / 32][64]: every lane's own pieces; all waves of a workgroup hold the same rows
     int limit[NC];         // tokens that the column sees
     int least, most;       // the smallest and largest limit of the wave's real columns
 
-    __device__ __forceinline__ void start(const AttnParams &p, const Request &rq, int head, int first_row) {
+    __device__ __forceinline__ void start(const AttnParams &p, const Request &rq, int head, int first_row, u32x4 *room) {
+        lds_q = room;
         const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
         const int cap = (int)min((int64_t)rq.len, (int64_t)p.width << p.shift);
         least = INT32_MAX;
@@ -295,7 +298,9 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
 #pragma unroll
             for (int s = 0; s < D / 32; ++s) {
                 const u32x4 x = *reinterpret_cast<const u32x4 *>(src + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
-                q[c][s] = real ? x : u32x4{0u, 0u, 0u, 0u};
+                const u32x4 y = real ? x : u32x4{0u, 0u, 0u, 0u};
+                if (kQueriesInLds) lds_q[(c * (D / 32) + s) * 64 + lane] = y;
+                else q[c][s] = y;
             }
             int lo = real ? limit[c] : INT32_MAX, hi = limit[c];
 #pragma unroll
@@ -347,18 +352,23 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
     __device__ __forceinline__ void scores(const KeyCodes<D, WIDE, STREAM> &k, f32x4 (&s)[NC][2]) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));        // the reads below stay in the loop: hoisted, the queries would take registers again
 #pragma unroll
         for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < 2; ++half) {
+                u32x4 b[NC];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) b[c] = kQueriesInLds ? lds_q[(c * (D / 32) + 2 * h + half) * 64 + lane] : q[kQueriesInLds ? 0 : c][2 * h + half];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const u32x4 a = {widen2<CODE, elem, 0>(k.c[t][h][2 * half]), widen2<CODE, elem, 1>(k.c[t][h][2 * half]),
                                      widen2<CODE, elem, 0>(k.c[t][h][2 * half + 1]), widen2<CODE, elem, 1>(k.c[t][h][2 * half + 1])};
 #pragma unroll
-                    for (int c = 0; c < NC; ++c)
-                        s[c][t] = mfma16x32(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, q[c][2 * h + half]), s[c][t]);
+                    for (int c = 0; c < NC; ++c) s[c][t] = mfma16x32(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b[c]), s[c][t]);
                 }
+            }
     }
 
     __device__ __forceinline__ void weigh(f32x4 (&s)[NC][2], float f, ValueCodes<D, WIDE, STREAM> &v, bool held, int t0) {

@@ -12,6 +12,7 @@ template <int CODE, int D, int NC, int W, bool WIDE, bool STREAM>
 __global__ void __launch_bounds__(W * 64) paged_decode_kernel(const AttnParams p) {
     constexpr int kRows = 16 * NC;
     __shared__ float lds_ml[W][kRows][2];
+    __shared__ u32x4 lds_q[NC > 1 ? NC * (D / 32) * 64 : 1];
     extern __shared__ float lds_o[];                       // [W/2][kRows][D]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i = lane & 15;
     const int head = blockIdx.x % p.heads, item = blockIdx.x / p.heads;
@@ -26,7 +27,7 @@ __global__ void __launch_bounds__(W * 64) paged_decode_kernel(const AttnParams p
     pages.fill(p, row, t0, 32 * W);
     const Request rq = request_of(p, it.r);
     Walk<CODE, D, NC, WIDE, STREAM> walk;
-    walk.start(p, rq, head, it.tile * kRows);
+    walk.start(p, rq, head, it.tile * kRows, lds_q);
     const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
     walk.run(p, row, pages, head, t0, 32 * W, end);
     walk.finish();

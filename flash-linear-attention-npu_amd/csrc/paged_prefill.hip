@@ -8,8 +8,9 @@ namespace fla {
 namespace {
 
 template <int CODE, int D, int NC, bool WIDE>
-__global__ void __launch_bounds__(64) paged_prefill_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(64, 2) paged_prefill_kernel(const AttnParams p) {
     constexpr int kRows = 16 * NC;
+    __shared__ u32x4 lds_q[NC * (D / 32) * 64];
     const int head = blockIdx.x % p.heads;
     if (p.clear_tail && blockIdx.x < p.heads) clear_tail<64>(p, head, D);
     int base;
@@ -23,7 +24,7 @@ __global__ void __launch_bounds__(64) paged_prefill_kernel(const AttnParams p) {
     pages.fill(p, row, t0, 32);
     const Request rq = request_of(p, it.r);
     Walk<CODE, D, NC, WIDE, false> walk;
-    walk.start(p, rq, head, it.tile * kRows);
+    walk.start(p, rq, head, it.tile * kRows, lds_q);
     const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
     walk.run(p, row, pages, head, t0, 32, end);
     walk.finish();
