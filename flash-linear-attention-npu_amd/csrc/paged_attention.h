@@ -267,15 +267,19 @@ template <int D, bool WIDE, bool STREAM> struct ValueCodes {
 //    p vs / r with r the largest v scale so far (the accumulators are kept in units of r), rounded to fp16 with 11 bits:
 //    a bf16 weight would add an error as large as the rounding of the result.  vs / r enters as an addend of the
 //    exponent, which costs nothing for each element; pages whose scale is 0 or below r 2^-20 take a product instead.
-//  - the maximum moves only when a score passes it by 2^8 (weights then stay below 2^8, far inside fp16), so most steps
-//    need no exchange between lanes and no rescaling.
-// The next step's keys are loaded as soon as this step's are consumed, its values likewise.  Sums and statistics are fp32.
+//  - the maximum moves only when the eight weights of a lane sum to more than 2^11 (fp16 holds 2^16), which the sum that is
+//    needed anyway tells, so most steps take no maximum, exchange nothing between lanes and rescale nothing.
+// STREAM (decode, memory far away): the next step's keys are loaded as soon as this step's are consumed, its values likewise.
+// Else (prefill, keys in L2): values are loaded ahead of the first product and keys ahead of the second, which leaves 32
+// registers more, and room for two waves on a SIMD.  Sums and statistics are fp32.
 template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
     typedef elemx8 T8;
-    static constexpr float kMoveMax = 8.f, kFold = 0x1p-20f;
+    static constexpr float kMost = 0x1p11f, kFold = 0x1p-20f, kLeast = 0x1p-100f;
     f32x4 o[NC][D / 16];   // o[c][j][e] of lane (g, i): channel D/16 (4 g + e) + j of query row 16 c + i, in units of r
-    float m[NC], l[NC];    // maximum in log2 (the same in all lanes of a column), this lane's share of the sum
-    float r;
+    float m[NC], l[NC];    // the largest score in log2 when it last moved (the same in all lanes of a column), this lane's share of the sum
+    float r, log_r;        // log2 of r
+    unsigned seen;         // bit c: the column has seen a token
+    bool fresh;
     static constexpr bool kQueriesInLds = NC > 1;
     u32x4 q[kQueriesInLds ? 1 : NC][D / 32];
     u32x4 *lds_q;          // [NC][D / 32][64]: every lane's own pieces; all waves of a workgroup hold the same rows
@@ -288,7 +292,9 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         const int cap = (int)min((int64_t)rq.len, (int64_t)p.width << p.shift);
         least = INT32_MAX;
         most = 0;
-        r = 0.f;
+        r = log_r = 0.f;
+        seen = 0;
+        fresh = true;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int row = first_row + 16 * c + i, tok = row / p.group, h = head * p.group + row - tok * p.group;
@@ -310,8 +316,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
             }
             least = min(least, lo);
             most = max(most, hi);
-            m[c] = kNegInf;
-            l[c] = 0.f;
+            m[c] = l[c] = 0.f;
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) o[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
@@ -330,20 +335,23 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         ValueCodes<D, WIDE, STREAM> v;
         Place<WIDE> at = pages.get(p, row, t0, stride, 0, most);
         k.load(p, head, t0, at, off);
-        v.load(p, head, t0, at, off);
+        if (STREAM) v.load(p, head, t0, at, off);
         for (int step = 1;; ++step) {
             const int t1 = t0 + stride;
+            const bool go = t1 < end;
             f32x4 s[NC][2];
+            Place<WIDE> next = at;
+            if (!STREAM) v.load(p, head, t0, at, off);
             scores(k, s);
             const float f = k.scale * p.scale2;
-            Place<WIDE> next = at;
-            if (t1 < end) {
-                next = pages.get(p, row, t1, stride, step, most);
-                k.load(p, head, t1, next, off);
-            }
-            weigh(s, f, v, at.held, t0);
-            if (t1 >= end) break;
-            v.load(p, head, t1, next, off);
+            if (go) next = pages.get(p, row, t1, stride, step, most);
+            if (STREAM && go) k.load(p, head, t1, next, off);
+            f16x8 w[NC];
+            weigh(s, f, v, at.held, t0, w);
+            if (!STREAM && go) k.load(p, head, t1, next, off);
+            accumulate(v, w);
+            if (!go) break;
+            if (STREAM) v.load(p, head, t1, next, off);
             at = next;
             t0 = t1;
         }
@@ -371,11 +379,44 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
             }
     }
 
-    __device__ __forceinline__ void weigh(f32x4 (&s)[NC][2], float f, ValueCodes<D, WIDE, STREAM> &v, bool held, int t0) {
+    // Moves the maximum of a column to its largest score so far; `by`: what its sum and accumulators are to be multiplied by.
+    // A column that has seen nothing keeps a maximum of 0 (its scores are -inf, its weights 0).
+    __device__ __forceinline__ void settle(const f32x4 (&s)[2], float f, int c, float &by) {
+        float best = kNegInf;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) best = fmaxf(best, s[t][e] * f);
+        best = fmaxf(best, __shfl_xor(best, 16, kWave));
+        best = fmaxf(best, __shfl_xor(best, 32, kWave));
+        const bool any = best > kNegInf, first = !(seen & (1u << c));
+        const float top = !any ? m[c] : first ? best : fmaxf(best, m[c]);
+        by = first ? 1.f : by * __builtin_amdgcn_exp2f(m[c] - top);                     // first: sum and accumulators are 0
+        m[c] = top;
+        seen |= any ? 1u << c : 0u;
+    }
+
+    // Eight weights of a column in the operand's order and their sum (before `ratio`).
+    __device__ __forceinline__ f16x8 exponentials(const f32x4 (&s)[2], float f, float bias, float &sum, float ratio = 1.f) {
+        u32x4 packed;
+        f32x2 part[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[t][e], f, bias)), __builtin_amdgcn_exp2f(fmaf(s[t][e + 1], f, bias))};
+                part[2 * t + e / 2] = x;
+                packed[2 * t + e / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x[0] * ratio, x[1] * ratio}, f16x2v));
+            }
+        sum = ((part[0][0] + part[0][1]) + (part[1][0] + part[1][1])) + ((part[2][0] + part[2][1]) + (part[3][0] + part[3][1]));
+        return __builtin_bit_cast(f16x8, packed);
+    }
+
+    __device__ __forceinline__ void weigh(f32x4 (&s)[NC][2], float f, ValueCodes<D, WIDE, STREAM> &v, bool held, int t0, f16x8 (&w)[NC]) {
         const int tok = t0 + 8 * (int)((threadIdx.x & 63) >> 4);
         const bool masked = t0 + 32 > least || __any(!held);      // some column does not see all of the step
         bool nan = false;
-        if (masked) {
+        if (__builtin_expect(masked, 0)) {
             bool mine = false;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -394,82 +435,51 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
                     for (int e = 0; e < 4; ++e) s[c][t][e] = tok + 4 * t + e < limit[c] && held ? s[c][t][e] * f : kNegInf;
             f = 1.f;
         }
-        bool move = false;
-        const bool negative = __any(f < 0.f);
+        float by[NC], by_r = 1.f;          // what sums, and beyond that accumulators, are multiplied by
+        bool moved = false;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            float best = fmaxf(fmaxf(fmaxf(s[c][0][0], s[c][0][1]), fmaxf(s[c][0][2], s[c][0][3])), fmaxf(fmaxf(s[c][1][0], s[c][1][1]), fmaxf(s[c][1][2], s[c][1][3])));
-            if (negative && f < 0.f) best = fminf(fminf(fminf(s[c][0][0], s[c][0][1]), fminf(s[c][0][2], s[c][0][3])), fminf(fminf(s[c][1][0], s[c][1][1]), fminf(s[c][1][2], s[c][1][3])));
-            move = move || best * f > m[c] + kMoveMax;
-        }
-        if (__any(move)) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float best = m[c];
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) best = fmaxf(best, s[c][t][e] * f);
-                best = fmaxf(best, __shfl_xor(best, 16, kWave));
-                best = fmaxf(best, __shfl_xor(best, 32, kWave));
-                const float by = best == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[c] - best);   // 0 before the first token
-                m[c] = best;
-                l[c] *= by;
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) o[c][j] *= by;
-            }
-        }
-        if (__any(v.scale > r)) {
+        for (int c = 0; c < NC; ++c) by[c] = 1.f;
+        if (__builtin_expect(__any(v.scale > r), 0)) {
             float top = fmaxf(r, v.scale);
             if (!WIDE) {
                 top = fmaxf(top, __shfl_xor(top, 16, kWave));
                 top = fmaxf(top, __shfl_xor(top, 32, kWave));
             }
-            const float by = r / top;
+            by_r = r / top;
             r = top;
+            log_r = __builtin_amdgcn_logf(top);
+            moved = true;
+        }
+        const bool fold = !__any(held && !(v.scale >= r * kFold && v.scale >= kLeast)), early = masked || fresh || !fold;
+        const float add = fold && held ? __builtin_amdgcn_logf(v.scale) - log_r : 0.f;
+        const float back = fold && held ? r * __builtin_amdgcn_rcpf(v.scale) : 1.f, ratio = fold ? 1.f : r > 0.f ? v.scale / r : 0.f;
+        moved = moved || early;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float sum;
+            if (__builtin_expect(early, 0)) settle(s[c], f, c, by[c]);
+            w[c] = exponentials(s[c], f, add - m[c], sum);
+            if (__builtin_expect(__any(sum > kMost), 0)) {
+                settle(s[c], f, c, by[c]);
+                moved = true;
+                w[c] = exponentials(s[c], f, add - m[c], sum);
+            }
+            if (__builtin_expect(!fold, 0)) w[c] = exponentials(s[c], f, -m[c], sum, ratio);
+            l[c] = fmaf(sum, back, l[c] * by[c]);
+        }
+        if (__builtin_expect(fresh, 0)) {
+            bool none = false;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) none = none || (limit[c] > 0 && !(seen & (1u << c)));
+            fresh = __any(none);
+        }
+        if (__builtin_expect(moved, 0)) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int j = 0; j < D / 16; ++j) o[c][j] *= by;
+                for (int j = 0; j < D / 16; ++j) o[c][j] *= by[c] * by_r;
         }
-        f16x8 w[NC];
-        if (!__any(held && !(v.scale >= r * kFold && r > 0.f))) {
-            const float add = held ? __builtin_amdgcn_logf(v.scale / r) : 0.f, back = held ? r / v.scale : 1.f;   // log2
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const float bias = add - (m[c] == kNegInf ? 0.f : m[c]);      // nothing seen yet: every weight is exp2(-inf) = 0
-                float sum = 0.f;
-                u32x4 packed;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[c][t][e], f, bias)), __builtin_amdgcn_exp2f(fmaf(s[c][t][e + 1], f, bias))};
-                        sum += x[0] + x[1];
-                        packed[2 * t + e / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(x, f16x2v));
-                    }
-                l[c] = fmaf(sum, back, l[c]);
-                w[c] = __builtin_bit_cast(f16x8, packed);
-            }
-        } else {
-            const float ratio = r > 0.f ? v.scale / r : 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const float bias = m[c] == kNegInf ? 0.f : -m[c];
-                u32x4 packed;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        const f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[c][t][e], f, bias)), __builtin_amdgcn_exp2f(fmaf(s[c][t][e + 1], f, bias))};
-                        l[c] += x[0] + x[1];
-                        packed[2 * t + e / 2] = __builtin_bit_cast(unsigned, __builtin_convertvector(x * ratio, f16x2v));
-                    }
-                w[c] = __builtin_bit_cast(f16x8, packed);
-            }
-        }
-        if (nan) spread_nan(v, tok, held);
-        accumulate(v, w);
+        if (__builtin_expect(nan, 0)) spread_nan(v, tok, held);
     }
 
     // A NaN in a token that some columns see and others do not: put into the columns that see it, taken out of the codes.
@@ -532,6 +542,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         for (int c = 0; c < NC; ++c) {
             l[c] += __shfl_xor(l[c], 16, kWave);
             l[c] += __shfl_xor(l[c], 32, kWave);
+            if (l[c] == 0.f) m[c] = kNegInf;
         }
     }
 

@@ -9,11 +9,11 @@ namespace fla {
 namespace {
 
 template <int CODE, int D, int NC, int W, bool WIDE, bool STREAM>
-__global__ void __launch_bounds__(W * 64) paged_decode_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(W * 64, 2) paged_decode_kernel(const AttnParams p) {
     constexpr int kRows = 16 * NC;
     __shared__ float lds_ml[W][kRows][2];
     __shared__ u32x4 lds_q[NC > 1 ? NC * (D / 32) * 64 : 1];
-    extern __shared__ float lds_o[];                       // [W/2][kRows][D]
+    __shared__ f32x4 lds_o[W / 2][D / 16 * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i = lane & 15;
     const int head = blockIdx.x % p.heads, item = blockIdx.x / p.heads;
     if (p.clear_tail && blockIdx.x >= gridDim.x - p.heads) clear_tail<W * 64>(p, head, D);
@@ -55,25 +55,22 @@ __global__ void __launch_bounds__(W * 64) paged_decode_kernel(const AttnParams p
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) walk.o[c][j] *= by;
     }
+    // one column tile at a time, so that the room does not keep other workgroups off the compute unit
 #pragma unroll
-    for (int half = W / 2; half >= 1; half >>= 1) {
-        if (wave >= half && wave < 2 * half) {
-            f32x4 *dst = reinterpret_cast<f32x4 *>(lds_o + (size_t)(wave - half) * kRows * D);
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+        for (int half = W / 2; half >= 1; half >>= 1) {
+            if (wave >= half && wave < 2 * half) {
 #pragma unroll
-                for (int j = 0; j < D / 16; ++j) dst[(c * (D / 16) + j) * 64 + lane] = walk.o[c][j];
+                for (int j = 0; j < D / 16; ++j) lds_o[wave - half][j * 64 + lane] = walk.o[c][j];
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) walk.o[c][j] += lds_o[wave][j * 64 + lane];
+            }
+            if (half > 1 || c + 1 < NC) __syncthreads();
         }
-        __syncthreads();
-        if (wave < half) {
-            const f32x4 *src = reinterpret_cast<const f32x4 *>(lds_o + (size_t)wave * kRows * D);
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int j = 0; j < D / 16; ++j) walk.o[c][j] += src[(c * (D / 16) + j) * 64 + lane];
-        }
-        if (half > 1) __syncthreads();
-    }
     if (wave == 0) walk.store(p, rq, it, item, head, kRows, 0, m, l);
 }
 
@@ -166,10 +163,7 @@ __global__ void __launch_bounds__(64 * (WAVES > 4 ? WAVES : 4)) paged_join_kerne
 
 template <int CODE, int D, int NC, int W, bool WIDE, bool STREAM> int launch(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
     const dim3 grid((unsigned)(plan.items * p.heads));
-    const size_t lds = (size_t)(W / 2) * 16 * NC * D * 4;
-    const auto kernel = paged_decode_kernel<CODE, D, NC, W, WIDE, STREAM>;
-    if (lds > 48 * 1024) FLA_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    FLA_LAUNCH("paged_kv_attention", stream, kernel, grid, dim3(W * 64), lds, stream, p);
+    FLA_LAUNCH("paged_kv_attention", stream, (paged_decode_kernel<CODE, D, NC, W, WIDE, STREAM>), grid, dim3(W * 64), 0, stream, p);
     FLA_HIP_CHECK(hipGetLastError());
     return FLA_OK;
 }
@@ -178,9 +172,6 @@ template <int CODE, int D, bool WIDE> int launch_rows(const AttnParams &p, const
     if (plan.nc == 1) {
         if (plan.waves == 8) return launch<CODE, D, 1, 8, WIDE, false>(p, plan, stream);
         return launch<CODE, D, 1, 4, WIDE, true>(p, plan, stream);
-    }
-    if constexpr (D <= 128) {
-        if (plan.nc == 4) return launch<CODE, D, 4, 4, WIDE, true>(p, plan, stream);
     }
     return launch<CODE, D, 2, 4, WIDE, true>(p, plan, stream);
 }
