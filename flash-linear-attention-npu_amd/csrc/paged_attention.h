@@ -26,7 +26,9 @@ struct AttnParams {
     int64_t q_t, q_h, o_t, o_h, lse_t, lse_h, kc_p, kc_h, kc_t, vc_p, vc_h, vc_t, ks_p, ks_h, vs_p, vs_h, table_s;
     int tokens, n, width, shift, group, heads;
     uint32_t pool;
-    int target, min_units;         // items wanted; shortest chunk in units; target 0: one chunk for each tile
+    // Chunk length: long enough for about `few` items, or shorter where chunks of 16 units and about `target` items allow it;
+    // at least min_units.  target 0: one chunk for each tile.
+    int target, few, min_units;
     int tiles_each;                // tiles of a request without cu
     float scale2;                  // scale * log2(e)
     bool clear_tail;
@@ -101,7 +103,8 @@ template <int ROWS> __device__ __forceinline__ Item find_item(const AttnParams &
         // sum over the lanes in two halves; one more than the quotient, so that rounding cannot make more items than the grid
         const int lo = __builtin_amdgcn_readlane(wave_scan((int)(work & 0xffff)), 63), hi = __builtin_amdgcn_readlane(wave_scan((int)(work >> 16)), 63);
         const float all = (float)hi * 65536.f + (float)lo;
-        it.units = max((int)fminf(all / (float)p.target, 1e9f) + 1, p.min_units);
+        const int most = (int)fminf(all / (float)p.few, 1e9f) + 1, least = (int)fminf(all / (float)p.target, 1e9f) + 1;
+        it.units = max(min(most, max(least, 16)), p.min_units);
     }
     int items_before = 0, tiles_before = 0;
     for (int r0 = 0; r0 < p.n; r0 += kWave) {

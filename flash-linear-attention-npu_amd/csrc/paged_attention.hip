@@ -64,17 +64,19 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
     plan.tiles = present(cu) ? T * group / rows + n : n * ((group + rows - 1) / rows);
     p.tiles_each = (int)((group + rows - 1) / rows);
     // The split of the key axis.  Lengths are on the device; the host knows the most that a row of the table can name.
-    //  - decode: chunks of at least 256 tokens; about 512 workgroups where there are few tiles, 2048 where tiles alone fill
-    //    the chip, since ragged requests balance better (32 heads on 8 of 128, e4m3: one request of 262 k tokens 102 us with
-    //    512 and 115 us with 2048 workgroups; 128 requests of up to 8 k 239 and 211 us);
+    //  - decode: about 512 workgroups (of chunks of at least 256 tokens) where there are few tiles; up to 2048, of chunks of at
+    //    least 1024 tokens, where tiles alone fill the chip, since ragged requests balance better (32 heads on 8 of 128,
+    //    e4m3: one request of 262 k tokens 102 us with 512 and 115 us with 2048 workgroups; 128 requests of up to 8 k 239
+    //    and 211 us);
     //  - tables of at most 2048 tokens: one chunk and one launch, of eight waves (four requests of 1100: 11.8 us against 12 us
     //    with two launches on the GPU, and one launch less on the host);
-    //  - prefill: only where tiles would leave compute units idle.
+    //  - prefill: only where tiles, of one wave each, would leave compute units idle.
     const int64_t capacity = table->shape[1] << shape.shift, tiles_all = plan.tiles * shape.heads;
     plan.waves = 4;
     p.min_units = 4;
-    p.target = (int)(((prefill ? 1024 : tiles_all < 256 ? 512 : 2048) + shape.heads - 1) / shape.heads);
-    if (prefill ? tiles_all >= 1024 : capacity <= 2048) {
+    p.target = (int)(((!prefill && tiles_all < 256 ? 512 : 2048) + shape.heads - 1) / shape.heads);
+    p.few = prefill ? p.target : (int)((512 + shape.heads - 1) / shape.heads);
+    if (prefill ? tiles_all >= 2048 : capacity <= 2048) {
         p.target = 0;
         if (plan.nc == 1 && tiles_all < 512) plan.waves = 8;
     }

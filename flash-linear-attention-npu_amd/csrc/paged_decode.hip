@@ -9,7 +9,7 @@ namespace fla {
 namespace {
 
 template <int CODE, int D, int NC, int W, bool WIDE, bool STREAM>
-__global__ void __launch_bounds__(W * 64, 2) paged_decode_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(W * 64, NC == 2 && D == 128 ? 3 : 2) paged_decode_kernel(const AttnParams p) {
     constexpr int kRows = 16 * NC;
     __shared__ float lds_ml[W][kRows][2];
     __shared__ u32x4 lds_q[NC > 1 ? NC * (D / 32) * 64 : 1];
