@@ -3,7 +3,7 @@
 //   table[r, old_r + j] = free[base_r + j];  token t of request r: position c_r + t - cu_r, slot = page * P + offset
 // A few kilobytes for a decode step: bound by latency, so the whole plan is ONE launch.  Every workgroup scans all
 // lengths for itself (two prefix sums over tiles of 1024 requests in LDS) instead of waiting for another one's sums, then
-// fills the 1024-token pieces and the 1024-entry pieces of new pages that fall to it; a token finds its request by
+// fills the pieces of 256 tokens and of 256 new pages that fall to it; a token finds its request by
 // bisection in the tile's sums.  A slot in a page that this step opens is computed from the free list, never read back
 // from the table, so no workgroup depends on another's writes.
 #include "common.h"
@@ -15,7 +15,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kPer = 4;                       // requests per thread and tile
 constexpr int kTile = kThreads * kPer;
-constexpr int kPiece = 1024;                  // tokens or new pages a workgroup takes at a time
+constexpr int kPiece = kThreads;              // tokens or new pages a workgroup takes at a time: one for each thread
 
 struct PlanParams {
     const int32_t *context, *query, *free_blocks, *state_rows;
@@ -204,7 +204,7 @@ int plan_impl(const fla_tensor *context, const fla_tensor *query, const fla_tens
     p.used = static_cast<int32_t *>(used->data);
     p.state_indices = present(state_indices) ? static_cast<int32_t *>(state_indices->data) : nullptr;
     const int64_t pieces = (tokens + kPiece - 1) / kPiece;
-    const dim3 grid((unsigned)(pieces < 1 ? 1 : pieces > 512 ? 512 : pieces));
+    const dim3 grid((unsigned)(pieces < 1 ? 1 : pieces > 1024 ? 1024 : pieces));
     FLA_LAUNCH(op, stream, paged_kv_plan_kernel, grid, dim3(kThreads), 0, stream, p);
     FLA_HIP_CHECK(hipGetLastError());
     return FLA_OK;

@@ -72,17 +72,31 @@ def _wrap_mutable_op(name: str, op: Callable) -> Callable:
     declared = MUTATED_ARGUMENTS.get(name, ())
     if not declared:
         return op
-    parameters = inspect.signature(op)
+    parameters = inspect.signature(op).parameters
+    # where a declared argument stands in a call: bound by hand, since Signature.bind takes as long as a small launch
+    places = {name: (index, None if parameter.default is inspect.Parameter.empty else parameter.default)
+              for index, (name, parameter) in enumerate(parameters.items())}
     writes_this_call = MUTATION_PREDICATES.get(name)
+
+    class Arguments:
+        __slots__ = ("args", "kwargs")
+
+        def __init__(self, args, kwargs):
+            self.args, self.kwargs = args, kwargs
+
+        def __getitem__(self, arg):
+            if arg in self.kwargs:
+                return self.kwargs[arg]
+            index, default = places[arg]
+            return self.args[index] if index < len(self.args) else default
 
     @functools.wraps(op)
     def guarded(*args, **kwargs):
         import torch
 
-        call = parameters.bind(*args, **kwargs)
-        call.apply_defaults()
-        written = declared if writes_this_call is None or writes_this_call(call.arguments) else ()
-        targets = {arg: call.arguments[arg] for arg in written}
+        arguments = Arguments(args, kwargs)
+        written = declared if writes_this_call is None or writes_this_call(arguments) else ()
+        targets = {arg: arguments[arg] for arg in written}
         blocked = [arg for arg, value in targets.items() if getattr(value, "requires_grad", False)]
         if blocked:
             raise RuntimeError(

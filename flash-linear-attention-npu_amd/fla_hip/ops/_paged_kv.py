@@ -25,11 +25,11 @@ OP_ARGTYPES = {
     "paged_kv_attention": [_VP] * 8 + [_F64, _I64, _B, _VP, _VP],
 }
 
-_FLA_TENSOR = struct.Struct("Pii8q8q")
+# fla_tensor of each rank: pointer, type, rank, extents and strides, each padded to eight
+_FLA_TENSOR = tuple(struct.Struct(f"Pii{n}q{8 * (8 - n)}x{n}q{8 * (8 - n)}x") for n in range(_runtime.FLA_MAX_DIMS + 1))
 _CODES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2, "torch.int32": 3, "torch.int64": 4, "torch.int8": 5,
           "torch.float8_e4m3fn": 6}
 _CODE_OF = {}     # torch.dtype -> fla_dtype
-_ZEROS = tuple((0,) * (_runtime.FLA_MAX_DIMS - n) for n in range(_runtime.FLA_MAX_DIMS + 1))
 
 
 class _Call:
@@ -59,16 +59,13 @@ class _Call:
         n = len(shape)
         if n > _runtime.FLA_MAX_DIMS:
             raise ValueError(f"{name} has rank {n} > {_runtime.FLA_MAX_DIMS}.")
-        pad = _ZEROS[n]
-        return _FLA_TENSOR.pack(ptr, code, n, *shape, *pad, *stride, *pad)
+        return _FLA_TENSOR[n].pack(ptr, code, n, *shape, *stride)
 
     def run(self, name: str, *args):
         """``fla_<name>(<operands>, stream)`` on the current stream of the call's device."""
-        import torch
-
         launch = _runtime.bind_direct(name, OP_ARGTYPES[name])
         with _runtime.device_guard(self.device):
-            status = launch(*args, torch.cuda.current_stream(self.device).cuda_stream)
+            status = launch(*args, _runtime.raw_stream(self.device))
         if status:
             raise RuntimeError(f"fla_{name} failed with status={status}: {_runtime.last_error()}")
 
@@ -83,8 +80,7 @@ class _Call:
             if status:
                 raise RuntimeError(f"fla_{name}_get_workspace_size failed with status={status}: {_runtime.last_error()}")
             workspace = torch.empty(size.value, dtype=torch.uint8, device=self.device) if size.value else None
-            status = launch(*args, workspace.data_ptr() if workspace is not None else None, size.value,
-                            torch.cuda.current_stream(self.device).cuda_stream)
+            status = launch(*args, workspace.data_ptr() if workspace is not None else None, size.value, _runtime.raw_stream(self.device))
         if status:
             raise RuntimeError(f"fla_{name} failed with status={status}: {_runtime.last_error()}")
 
@@ -123,9 +119,10 @@ def paged_kv_plan(context_lens, query_lens, block_table, free_blocks, block_size
         raise ValueError(f"paged_kv_plan: num_tokens must not be negative, got {num_tokens}.")
     n, dev, i32 = block_table.shape[0], call.device, torch.int32
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    positions = torch.empty(num_tokens, dtype=i32, device=dev)
-    cu, seq, used = torch.empty(n + 1, dtype=i32, device=dev), torch.empty(n, dtype=i32, device=dev), torch.empty(1, dtype=i32, device=dev)
-    states = None if state_rows is None else torch.empty(num_tokens, dtype=i32, device=dev)
+    # the int32 results are parts of one allocation
+    sizes = [num_tokens, n + 1, n, 1] if state_rows is None else [num_tokens, n + 1, n, 1, num_tokens]
+    positions, cu, seq, used, *rest = torch.empty(sum(sizes), dtype=i32, device=dev).split_with_sizes(sizes)
+    states = rest[0] if rest else None
     if n == 0:
         slots.fill_(-1)
         for t in (positions, cu, used):

@@ -223,6 +223,13 @@ def device_guard(device):
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def raw_stream(device) -> int:
+    """The ``hipStream_t`` of torch's current stream on ``device``, without making a ``torch.cuda.Stream`` for it."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def call_op_noalloc(name: str, argtypes: Sequence, build_args: Callable[[CallContext], list], outputs):
     """One-phase call of ``fla_<name>(<operands>, stream)``: an entry point that brings its own scratch memory.
     Nothing is allocated here or inside the library; the caller has allocated ``outputs``."""
