@@ -187,6 +187,30 @@ def causal_conv1d(x, weight, bias=None, conv_states=None, *, query_start_loc=Non
     return Function.apply(x, weight, bias, conv_states)
 
 
+@functools.lru_cache(maxsize=1)
+def _rotary_function():
+    import torch
+
+    class RotaryAxes(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, positions, inv_freq, sections, axis_order, pairing):
+            ctx.save_for_backward(positions, inv_freq)
+            ctx.how = sections, axis_order, pairing
+            ctx.set_materialize_grads(False)
+            return _paged_kv._rotate(q, k, positions, inv_freq, sections, axis_order, pairing, False)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, dq, dk):
+            grads = [g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk)]
+            if grads[0] is None:
+                grads = [None if grads[1] is None else _paged_kv._rotate(grads[1], None, *ctx.saved_tensors, *ctx.how, True)[0]]
+                return None, *grads, *[None] * 5
+            return *_paged_kv._rotate(*grads, *ctx.saved_tensors, *ctx.how, True), *[None] * 5
+
+    return RotaryAxes
+
+
 def rotary_axes(q, k, positions, inv_freq, sections, *, axis_order="blocked", pairing="half"):
     """Rotary positions with one or more axes (text; height and width; time, height and width), differentiable in q and k.
 
@@ -196,28 +220,9 @@ def rotary_axes(q, k, positions, inv_freq, sections, *, axis_order="blocked", pa
     axes in turn while they have any left (``"interleaved"``).  Channel pair j turns by ``positions[axis_j] * inv_freq[j]``
     (formed in 64 bits); a pair is channels j and j + R/2 (``pairing="half"``) or 2j and 2j + 1 (``"adjacent"``).  Channels
     from R on pass through.  Returns the rotated q and k in the memory order of the inputs."""
-    import torch
-
-    how = dict(axis_order=axis_order, pairing=pairing)
-    if not _has_tensor_requiring_grad(q, k):
-        return rotary_axes_fwd(q, k, positions, inv_freq, sections, **how)
-
-    class Function(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, q_, k_):
-            ctx.save_for_backward(positions, inv_freq)
-            return rotary_axes_fwd(q_, k_, positions, inv_freq, sections, **how)
-
-        @staticmethod
-        @torch.autograd.function.once_differentiable
-        def backward(ctx, dq, dk):
-            turned = ctx.saved_tensors
-            grads = [None if g is None else g if g.stride(-1) == 1 else g.contiguous() for g in (dq, dk)]
-            if grads[0] is None:
-                return None, rotary_axes_bwd(grads[1], None, *turned, sections, **how)[0]
-            return rotary_axes_bwd(*grads, *turned, sections, **how)
-
-    return Function.apply(q, k)
+    if _has_tensor_requiring_grad(q, k):
+        return _rotary_function().apply(q, k, positions, inv_freq, sections, axis_order, pairing)
+    return _paged_kv._rotate(q, k, positions, inv_freq, sections, axis_order, pairing, False)
 
 
 __all__ = [

@@ -1,0 +1,319 @@
+"""Host-side contract of the paged 8-bit attention operators, without a GPU: what the entry points refuse, workspace sizes,
+the front end's checks, and the oracle against closed forms and torch's own 8-bit conversion.  Nothing is launched."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from oracle import paged_kv as ref
+
+F32, F16, BF16, I32, I64, I8, F8 = range(7)
+OK, NULL, DTYPE, SHAPE, UNSUPPORTED, WORKSPACE = range(6)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import fla_hip
+
+    return fla_hip.load_library()
+
+
+def desc(shape, dtype, strides=None, data=4096):
+    """A packed descriptor of memory that is never touched."""
+    from fla_hip.ops import _paged_kv as P
+
+    if strides is None:
+        strides, n = [], 1
+        for d in reversed(shape):
+            strides.insert(0, n)
+            n *= d
+    return P._FLA_TENSOR[len(shape)].pack(data, dtype, len(shape), *shape, *strides)
+
+
+def test_packed_descriptors_are_the_structure_of_the_header():
+    from fla_hip.ops._runtime import FlaTensor
+
+    packed = FlaTensor.from_buffer_copy(desc((2, 3, 5), BF16, (40, 8, 1), data=123456))
+    assert (packed.data, packed.dtype, packed.ndim) == (123456, BF16, 3)
+    assert list(packed.shape) == [2, 3, 5, 0, 0, 0, 0, 0] and list(packed.stride) == [40, 8, 1, 0, 0, 0, 0, 0]
+    assert ctypes.sizeof(FlaTensor) == len(desc((1,), F32)) == len(desc((1,) * 8, F32))
+
+
+def attention_args(**change):
+    a = dict(query=desc((6, 8, 128), BF16), key_cache=desc((10, 2, 16, 128), F8), value_cache=desc((10, 2, 16, 128), F8),
+             key_scales=desc((10, 2), F32), value_scales=desc((10, 2), F32), block_table=desc((3, 4), I32), seq_lens=desc((3,), I32),
+             cu_seqlens=desc((4,), I32), scale=0.1, max_query_len=3, clear_tail=True, out=desc((6, 8, 128), BF16), lse=desc((6, 8), F32))
+    a.update(change)
+    return list(a.values())
+
+
+def query(lib, args):
+    from fla_hip.ops import _paged_kv as P
+
+    fn = lib.fla_paged_kv_attention_get_workspace_size
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["paged_kv_attention"], ctypes.POINTER(ctypes.c_uint64)], ctypes.c_int
+    size = ctypes.c_uint64(77)
+    return fn(*args, ctypes.byref(size)), size.value, lib.fla_last_error().decode()
+
+
+@pytest.mark.parametrize("change,status,text", [
+    (dict(query=None), NULL, "query must not be null"),
+    (dict(query=desc((6, 8, 128), F32)), DTYPE, "query has unsupported dtype"),
+    (dict(query=desc((6, 7, 128), BF16), out=desc((6, 7, 128), BF16)), SHAPE, "not a multiple"),
+    (dict(query=desc((6, 8, 64), BF16), out=desc((6, 8, 64), BF16)), SHAPE, "query has 64 channels"),
+    (dict(query=desc((6, 8, 128), BF16, (1028, 128, 1))), SHAPE, "16-byte aligned"),
+    (dict(query=desc((6, 8, 128), BF16, data=4100)), SHAPE, "16-byte aligned"),
+    (dict(query=desc((6, 8, 128), BF16, (-1024, 128, 1))), SHAPE, "rows of query"),
+    (dict(out=desc((6, 8, 128), F16)), DTYPE, "out has unsupported dtype"),
+    (dict(out=desc((6, 8, 128), BF16, (0, 128, 1))), SHAPE, "rows of out overlap"),
+    (dict(out=desc((5, 8, 128), BF16)), SHAPE, "shape of query"),
+    (dict(key_cache=desc((10, 2, 16, 128), BF16)), DTYPE, "key_cache has unsupported dtype"),
+    (dict(value_cache=desc((10, 2, 16, 128), I8)), SHAPE, "same shape and type"),
+    (dict(key_cache=desc((10, 2, 24, 128), F8), value_cache=desc((10, 2, 24, 128), F8)), UNSUPPORTED, "power of two from 16 to 256"),
+    (dict(key_cache=desc((10, 2, 8, 128), F8), value_cache=desc((10, 2, 8, 128), F8)), UNSUPPORTED, "power of two from 16 to 256"),
+    (dict(key_cache=desc((10, 2, 16, 96), F8), value_cache=desc((10, 2, 16, 96), F8)), UNSUPPORTED, "head size must be"),
+    (dict(key_cache=desc((10, 2, 16, 128), F8, (4096, 2048, 136, 1))), SHAPE, "16-byte aligned"),
+    (dict(key_cache=desc((10, 2, 16, 128), F8, (4096, 2048, 1, 16))), SHAPE, "rows of key_cache must be contiguous"),
+    (dict(key_cache=desc((10, 2, 16, 128), F8, (4096, 2048, 1 << 23, 1))), UNSUPPORTED, "too far apart"),
+    (dict(key_scales=desc((10, 3), F32)), SHAPE, "key_scales must be"),
+    (dict(value_scales=desc((10, 2), BF16)), DTYPE, "value_scales has unsupported dtype"),
+    (dict(block_table=desc((3, 4), I64)), DTYPE, "block_table has unsupported dtype"),
+    (dict(block_table=desc((3, 4), I32, (4, 2))), SHAPE, "unit innermost stride"),
+    (dict(block_table=desc((3, 1 << 28), I32)), SHAPE, "more than 2^31"),
+    (dict(seq_lens=desc((4,), I32)), SHAPE, "seq_lens must be"),
+    (dict(cu_seqlens=desc((3,), I32)), SHAPE, "cu_seqlens must be"),
+    (dict(cu_seqlens=None), SHAPE, "one row for each of the 3 requests"),
+    (dict(lse=desc((6, 7), F32)), SHAPE, "lse must be"),
+    (dict(max_query_len=-1), SHAPE, "must not be negative"),
+])
+def test_attention_refusals(lib, change, status, text):
+    got, _, message = query(lib, attention_args(**change))
+    assert got == status and text in message, (got, message)
+
+
+def test_attention_workspace(lib):
+    """Nothing for one chunk to a tile; else room for 2048 / heads items beyond the tiles, each of heads x rows x (D + 2) fp32."""
+    assert query(lib, attention_args())[:2] == (OK, 0)                       # the table names 64 tokens
+    wide = dict(block_table=desc((3, 1000), I32))
+    status, size, _ = query(lib, attention_args(**wide))
+    tiles = 6 * 4 // 16 + 3                                                   # 6 rows of 4 heads in tiles of 16, at most one more each
+    assert status == OK and size == (tiles + 256) * 2 * 16 * (128 + 2) * 4
+    assert query(lib, attention_args(**wide, cu_seqlens=None, query=desc((3, 8, 128), BF16), out=desc((3, 8, 128), BF16), lse=None))[1] == (3 + 256) * 2 * 16 * 130 * 4
+    assert query(lib, attention_args(lse=None))[0] == OK
+    from fla_hip.ops import _paged_kv as P
+
+    fn = lib.fla_paged_kv_attention
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["paged_kv_attention"], ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p], ctypes.c_int
+    assert fn(*attention_args(**wide), 4096, size - 1, None) == WORKSPACE     # refused before any launch
+    assert fn(*attention_args(**wide), None, size, None) == WORKSPACE
+
+
+def plan_args(**change):
+    a = dict(context=desc((3,), I32), query=desc((3,), I32), table=desc((3, 4), I32), free=desc((5,), I32), rows=desc((3,), I32), block=16,
+             slots=desc((7,), I64), positions=desc((7,), I32), cu=desc((4,), I32), seq=desc((3,), I32), used=desc((1,), I32), states=desc((7,), I32))
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,status,text", [
+    (dict(table=None), NULL, "block_table must not be null"),
+    (dict(table=desc((3, 4), I32, (2, 1))), SHAPE, "rows that do not overlap"),
+    (dict(context=desc((2,), I32)), SHAPE, "context_lens must have 3"),
+    (dict(query=desc((3,), I64)), DTYPE, "query_lens has unsupported dtype"),
+    (dict(query=desc((3,), I32, (2,))), SHAPE, "query_lens must be contiguous"),
+    (dict(free=None), NULL, "free_blocks"),
+    (dict(block=48), UNSUPPORTED, "power of two"),
+    (dict(slots=desc((7,), I32)), DTYPE, "slot_mapping has unsupported dtype"),
+    (dict(positions=desc((6,), I32)), SHAPE, "positions must have 7"),
+    (dict(cu=desc((3,), I32)), SHAPE, "cu_seqlens must have 4"),
+    (dict(states=None), NULL, "go together"),
+    (dict(rows=desc((2,), I32)), SHAPE, "state_rows must have 3"),
+])
+def test_plan_refusals(lib, change, status, text):
+    from fla_hip.ops import _paged_kv as P
+
+    fn = lib.fla_paged_kv_plan
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["paged_kv_plan"], ctypes.c_void_p], ctypes.c_int
+    assert fn(*plan_args(**change), None) == status and text in lib.fla_last_error().decode()
+
+
+def append_args(**change):
+    a = dict(key=desc((5, 2, 128), BF16), value=desc((5, 2, 128), BF16), kc=desc((10, 2, 16, 128), I8), vc=desc((10, 2, 16, 128), I8),
+             ks=desc((10, 2), F32), vs=desc((10, 2), F32), slots=desc((5,), I64))
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,status,text", [
+    (dict(key=desc((5, 3, 128), BF16)), SHAPE, "key must be [T,2,128]"),
+    (dict(value=desc((4, 2, 128), BF16)), SHAPE, "value must be"),
+    (dict(value=desc((5, 2, 128), F16)), DTYPE, "value has unsupported dtype"),
+    (dict(key=desc((5, 2, 128), BF16, (256, 130, 1))), SHAPE, "16-byte aligned"),
+    (dict(key=desc((5, 2, 128), BF16, (1 << 21, 128, 1))), UNSUPPORTED, "too far apart"),
+    (dict(slots=desc((5,), I32)), DTYPE, "slot_mapping has unsupported dtype"),
+    (dict(slots=desc((4,), I64)), SHAPE, "one slot for each row"),
+    (dict(vc=desc((10, 2, 16, 128), F8)), SHAPE, "same shape and type"),
+    (dict(kc=desc((0, 2, 16, 128), I8), vc=desc((0, 2, 16, 128), I8), ks=desc((0, 2), F32), vs=desc((0, 2), F32)), SHAPE, "at least one page"),
+])
+def test_append_refusals(lib, change, status, text):
+    from fla_hip.ops import _paged_kv as P
+
+    fn = lib.fla_paged_kv_append
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["paged_kv_append"], ctypes.c_void_p], ctypes.c_int
+    assert fn(*append_args(**change), None) == status and text in lib.fla_last_error().decode()
+
+
+def rotary_args(axes=(0, 0, 1, 1), **change):
+    from fla_hip.ops._runtime import FlaIntArray
+
+    data = (ctypes.c_int64 * len(axes))(*axes)
+    table = FlaIntArray(ctypes.cast(data, ctypes.POINTER(ctypes.c_int64)), len(axes))
+    a = dict(q=desc((5, 2, 16), BF16), k=desc((5, 1, 16), BF16), positions=desc((2, 5), I64), inv=desc((4,), F32), table=ctypes.addressof(table),
+             adjacent=False, inverse=False, q_out=desc((5, 2, 16), BF16), k_out=desc((5, 1, 16), BF16))
+    a.update(change)
+    return list(a.values()), (data, table)
+
+
+@pytest.mark.parametrize("axes,change,status,text", [
+    ((0, 0, 1, 2), {}, SHAPE, "names axis 2 of 2"),
+    ((0, 0, 1), {}, SHAPE, "one entry for each frequency"),
+    ((0,) * 9, dict(inv=desc((9,), F32)), SHAPE, "at most half as many"),
+    ((0, 0, 1, 1), dict(q=desc((5, 16), BF16)), SHAPE, "must be [B,T,H,D]"),
+    ((0, 0, 1, 1), dict(q=desc((5, 2, 16), I32)), DTYPE, "q has unsupported dtype"),
+    ((0, 0, 1, 1), dict(k=desc((5, 1, 16), F16)), DTYPE, "k has unsupported dtype"),
+    ((0, 0, 1, 1), dict(k=desc((4, 1, 16), BF16), k_out=desc((4, 1, 16), BF16)), SHAPE, "number of heads only"),
+    ((0, 0, 1, 1), dict(q=desc((5, 2, 16), BF16, (64, 32, 2))), SHAPE, "unit innermost stride"),
+    ((0, 0, 1, 1), dict(q_out=desc((5, 2, 16), BF16, (0, 16, 1))), SHAPE, "rows of an output overlap"),
+    ((0, 0, 1, 1), dict(q_out=desc((5, 3, 16), BF16)), SHAPE, "another shape"),
+    ((0, 0, 1, 1), dict(k_out=None), NULL, "go together"),
+    ((0, 0, 1, 1), dict(positions=desc((2, 6), I64)), SHAPE, "positions must be"),
+    ((0, 0, 1, 1), dict(positions=desc((2, 5), F32)), DTYPE, "positions has unsupported dtype"),
+    ((0, 0, 1, 1), dict(inv=desc((4,), F32, (2,))), SHAPE, "inv_freq must be contiguous"),
+    ((0,), dict(q=desc((5, 2, 15), BF16), q_out=desc((5, 2, 15), BF16), k=None, k_out=None, inv=desc((1,), F32)), SHAPE, "must be even"),
+])
+def test_rotary_refusals(lib, axes, change, status, text):
+    from fla_hip.ops import _paged_kv as P
+
+    fn = lib.fla_rotary_axes
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["rotary_axes"], ctypes.c_void_p], ctypes.c_int
+    args, keep = rotary_args(axes, **change)
+    assert fn(*args, None) == status and text in lib.fla_last_error().decode(), lib.fla_last_error()
+
+
+def test_front_end_refuses_cpu_tensors_and_bad_arguments():
+    from fla_hip import ops
+    from fla_hip.ops import _paged_kv as P
+
+    x = torch.zeros(2, 1, 64)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(TypeError, match="ROCm GPU tensor"):
+        ops.rotary_axes(x, None, i[None], torch.ones(4), (4,))
+    with pytest.raises(TypeError, match="ROCm GPU tensor"):
+        ops.paged_kv_plan(i, i, torch.zeros(2, 1, dtype=torch.int32), i, 16, 2)
+    with pytest.raises(TypeError, match="ROCm GPU tensor"):
+        ops.paged_kv_attention(x, x, x, x, x, i, i)
+    with pytest.raises(TypeError, match="ROCm GPU tensor"):
+        ops.paged_kv_append(x, x, x, x, x, x, i)
+    with pytest.raises(ValueError, match="axis_order must be"):
+        ops.rotary_axes(x, None, i[None], torch.ones(4), (4,), axis_order="mixed")
+    with pytest.raises(ValueError, match="pairing must be"):
+        ops.rotary_axes(x, None, i[None], torch.ones(4), (4,), pairing="none")
+    with pytest.raises(RuntimeError, match="paged_kv_append mutates key_cache in place"):
+        ops.paged_kv_append(x, x, x.clone().requires_grad_(), x, x, x, i)
+    with pytest.raises(RuntimeError, match="paged_kv_attention mutates out in place"):
+        ops.paged_kv_attention(x, x, x, x, x, i, i, out=x.clone().requires_grad_())
+    assert ops.MUTATED_ARGUMENTS["paged_kv_plan"] == ("block_table",)
+    assert [list(P._axis_table((3, 2, 1), o)[0]) for o in ("blocked", "interleaved")] == [[0, 0, 0, 1, 1, 2], [0, 1, 2, 0, 1, 0]]
+    for name in ("paged_kv_plan", "paged_kv_append", "paged_kv_attention", "rotary_axes", "rotary_axes_fwd", "rotary_axes_bwd"):
+        assert name in ops.__all__ and callable(getattr(ops, name))
+
+
+def test_mutation_guard_finds_arguments_by_place_and_by_name():
+    from fla_hip import ops
+
+    seen = []
+    guarded = ops._wrap_mutable_op("paged_kv_attention", lambda query, a, b, *, scale=None, out=None: seen.append((query, a, b, scale, out)) or "done")
+    out = torch.zeros(3)
+    assert guarded(1, 2, b=3, out=out) == "done" and out._version == 1 and seen[-1][2] == 3
+    assert guarded(1, 2, 3) == "done" and out._version == 1
+    with torch.inference_mode():
+        made = torch.zeros(3)
+    assert guarded(1, 2, 3, out=made) == "done"                               # no version counter to raise
+    by_place = ops._wrap_mutable_op("paged_kv_plan", lambda context, query, block_table, free: None)
+    by_place(1, 2, out, 4)
+    by_place(1, 2, block_table=out, free=4)
+    assert out._version == 3
+    with pytest.raises(TypeError):
+        by_place(1, 2)
+    with pytest.raises(RuntimeError, match="mutates block_table"):
+        by_place(1, 2, torch.zeros(2, requires_grad=True), 4)
+
+
+# ---- the oracle ------------------------------------------------------------------------------------------------------
+
+def test_oracle_codes_are_torch_conversions():
+    x = torch.cat([torch.randn(4000, dtype=torch.float64) * s for s in (1e-3, 0.1, 10, 300)] + [torch.tensor([0.0, 447.9, 448, 1e9, 2.0 ** -10, 3 * 2.0 ** -10, 2.0 ** -6], dtype=torch.float64)])
+    x = x.float().double()
+    want = x.clamp(-448, 448).float().to(torch.float8_e4m3fn).double()
+    assert torch.equal(ref.encode(x, torch.float8_e4m3fn), want)
+    assert ref.encode(torch.tensor([math.nan, math.inf, -math.inf], dtype=torch.float64), torch.float8_e4m3fn)[1:].tolist() == [448, -448]
+    assert ref.encode(torch.tensor([0.5, 1.5, -2.5, 200, math.nan], dtype=torch.float64), torch.int8).tolist() == [0, 2, -2, 127, 0]
+
+
+@pytest.mark.parametrize("dtype,most", [(torch.float8_e4m3fn, 448.0), (torch.int8, 127.0)])
+def test_oracle_scale_is_the_smallest_power_of_two(dtype, most):
+    assert ref.step_for(0.0, dtype) == 0 and ref.step_for(most, dtype) == 1 and ref.step_for(most * 1.0000001, dtype) == 2
+    for a in (1e-30, 0.37, 5.0, 3e38):
+        s = ref.step_for(a, dtype)
+        assert math.frexp(s)[0] == 0.5 and a / s <= most < a / (s / 2)
+
+
+def test_oracle_append_is_one_pass_over_a_page_in_pieces():
+    """Powers of two: filling a page row by row in e4m3 gives the codes of the whole page at once (normals)."""
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(16, 1, 64, generator=gen) + torch.sign(torch.randn(16, 1, 64, generator=gen))     # no subnormal codes
+    whole, step = torch.zeros(1, 1, 16, 64, dtype=torch.float64), torch.zeros(1, 1, dtype=torch.float64)
+    ref.append(x, whole, step, range(16), torch.float8_e4m3fn)
+    rows, by_row = torch.zeros_like(whole), torch.zeros_like(step)
+    for t in range(16):
+        ref.append(x[t:t + 1], rows, by_row, [t], torch.float8_e4m3fn)
+    assert torch.equal(whole, rows) and torch.equal(step, by_row)
+    assert float((whole[0, 0] * step[0, 0] - x[:, 0]).abs().max() / x.abs().max()) <= 2.0 ** -4
+
+
+def test_oracle_attention_is_softmax_attention():
+    gen = torch.Generator().manual_seed(1)
+    kc, vc = torch.randn(4, 2, 16, 64, generator=gen, dtype=torch.float64), torch.randn(4, 2, 16, 64, generator=gen, dtype=torch.float64)
+    ks, vs = torch.rand(4, 2, generator=gen), torch.rand(4, 2, generator=gen)
+    q = torch.randn(5, 4, 64, generator=gen)
+    table = torch.tensor([[2, 0, 3]])
+    out, lse, spread, _ = ref.attention(q, kc, vc, ks, vs, table, [37], [0, 5], 0.125)
+    k = (kc * ks.double()[..., None, None])[[2, 0, 3]].transpose(1, 2).flatten(0, 1)[:37].transpose(0, 1).repeat_interleave(2, 0)
+    v = (vc * vs.double()[..., None, None])[[2, 0, 3]].transpose(1, 2).flatten(0, 1)[:37].transpose(0, 1).repeat_interleave(2, 0)
+    mask = torch.arange(37) <= torch.arange(32, 37)[:, None]
+    want = torch.nn.functional.scaled_dot_product_attention(q.double().transpose(0, 1), k, v, attn_mask=mask, scale=0.125)
+    assert torch.allclose(out, want.transpose(0, 1), atol=1e-12) and bool((spread >= out.abs() - 1e-12).all())
+    score = (q.double().transpose(0, 1) @ k.transpose(-1, -2) * 0.125).masked_fill(~mask, -math.inf)
+    assert torch.allclose(lse, score.logsumexp(-1).t(), atol=1e-12)
+
+
+def test_oracle_rotary_keeps_norms_and_relative_angles():
+    gen = torch.Generator().manual_seed(2)
+    x, inv = torch.randn(7, 2, 12, generator=gen), torch.rand(5, generator=gen)
+    pos = torch.randint(0, 99, (2, 7), generator=gen)
+    for order in ("blocked", "interleaved"):
+        for pairing in ("half", "adjacent"):
+            y = ref.rotary(x, pos, inv, (3, 2), order, pairing)
+            assert torch.allclose(y.norm(dim=-1), x.double().norm(dim=-1)) and torch.equal(y[..., 10:], x[..., 10:].double())
+            back = ref.rotary(y, pos, inv, (3, 2), order, pairing, inverse=True)
+            assert torch.allclose(back, x.double(), atol=1e-12)
+            a, b = ref.rotary(x, pos + 5, inv, (3, 2), order, pairing), ref.rotary(x.flip(0), pos + 5, inv, (3, 2), order, pairing)
+            assert torch.allclose((a * b).sum(-1), (y * ref.rotary(x.flip(0), pos, inv, (3, 2), order, pairing)).sum(-1))
+
+
+def test_oracle_plan_closed_form():
+    table = [[4, -1], [7, -1]]
+    got = ref.plan([16, 3], [2, 15], table, [9, 8], 16, 18, [5, 6])
+    assert got["slots"].tolist() == [9 * 16, 9 * 16 + 1] + list(range(7 * 16 + 3, 7 * 16 + 16)) + [8 * 16, 8 * 16 + 1, -1]
+    assert got["table"].tolist() == [[4, 9], [7, 8]] and got["used"].tolist() == [2] and got["states"].tolist() == [5, 5] + [6] * 15 + [-1]
