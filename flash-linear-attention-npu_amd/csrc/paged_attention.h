@@ -132,7 +132,7 @@ template <int ROWS> __device__ __forceinline__ Item find_item(const AttnParams &
                 it.chunk = want - first_i - it.tile * it.chunks;
             }
             base = first_i + it.tile * it.chunks;
-            it.found = true;
+            it.found = it.tile >= 0 && it.tile < __builtin_amdgcn_readlane(tiles, l);   // false only where meaningless lengths overflowed the sums
             return it;
         }
         items_before = __builtin_amdgcn_readlane(end_i, 63);
@@ -258,6 +258,14 @@ template <int D, bool WIDE, bool STREAM> struct ValueCodes {
     }
 };
 
+// The power of two that the v scales of a request and head are measured in: that of its first page, if it has one.
+__device__ __forceinline__ float scale_unit(const AttnParams &p, const int32_t *table_row, int head) {
+    const int page = p.width ? table_row[0] : -1;
+    const float s = (uint32_t)page < p.pool ? p.vs[(int64_t)page * p.vs_p + head * p.vs_h] : 0.f;
+    if (!(s > 0.f && s < INFINITY)) return 0x1p-40f;
+    return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, fminf(fmaxf(s, 0x1p-60f), 0x1p60f)) & 0x7f800000u);
+}
+
 // One wave: 16 NC query rows against the tokens it is led over, 32 at a time.
 //   S^T = K Q^T: tokens are the rows of the accumulators, query rows their columns; O^T += V^T P^T with P^T straight from
 //   the accumulator layout.
@@ -266,10 +274,13 @@ template <int D, bool WIDE, bool STREAM> struct ValueCodes {
 //  - rows are given to tokens so that the accumulators of lane group g are tokens 8 g .. 8 g + 7 of the step: the
 //    contraction order of O^T.  V: lane 16 g + i loads D/16 neighbouring channels of those eight tokens, and a byte
 //    transpose inside the lane gives the operands of D/16 tiles whose row i is channel D/16 i + j of tile j.
-//  - scales of pages multiply S after the product (exact codes enter the matrix unit) and P: the weight of a token is
-//    p vs / r with r the largest v scale so far (the accumulators are kept in units of r), rounded to fp16 with 11 bits:
-//    a bf16 weight would add an error as large as the rounding of the result.  vs / r enters as an addend of the
-//    exponent, which costs nothing for each element; pages whose scale is 0 or below r 2^-20 take a product instead.
+//  - scales of pages multiply S after the product (exact codes enter the matrix unit).  The v scale enters the weight of a
+//    token as an addend of its exponent, w = 2^(s + log2(vs / u) - m), which costs nothing for each element; m is the
+//    largest s + log2(vs / u), so weights are measured against the largest contribution, whatever the scales of other
+//    pages are.  The sum of the softmax is that of w u / vs.  u, the scale of the request's first page as a power of two,
+//    only keeps these numbers inside fp32.  A scale below 2^-60 u (0 above all) counts as 2^-60 u in the exponent and
+//    multiplies the weight by the rest.
+//  - weights are rounded to fp16 with 11 bits: a bf16 weight would add an error as large as the rounding of the result.
 //  - the maximum moves only when the eight weights of a lane sum to more than 2^11 (fp16 holds 2^16), which the sum that is
 //    needed anyway tells, so most steps take no maximum, exchange nothing between lanes and rescale nothing.
 // STREAM (decode, memory far away): the next step's keys are loaded as soon as this step's are consumed, its values likewise.
@@ -277,10 +288,10 @@ template <int D, bool WIDE, bool STREAM> struct ValueCodes {
 // registers more, and room for two waves on a SIMD.  Sums and statistics are fp32.
 template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
     typedef elemx8 T8;
-    static constexpr float kMost = 0x1p11f, kFold = 0x1p-20f, kLeast = 0x1p-100f;
-    f32x4 o[NC][D / 16];   // o[c][j][e] of lane (g, i): channel D/16 (4 g + e) + j of query row 16 c + i, in units of r
-    float m[NC], l[NC];    // the largest score in log2 when it last moved (the same in all lanes of a column), this lane's share of the sum
-    float r, log_r;        // log2 of r
+    static constexpr float kMost = 0x1p11f;
+    f32x4 o[NC][D / 16];   // o[c][j][e] of lane (g, i): channel D/16 (4 g + e) + j of query row 16 c + i, in units of u 2^m
+    float m[NC], l[NC];    // the largest s + log2(vs / u) when it last moved (the same in all lanes of a column), this lane's share of the sum
+    float unit, log_unit;  // u, log2 u
     unsigned seen;         // bit c: the column has seen a token
     bool fresh;
     static constexpr bool kQueriesInLds = NC > 1;
@@ -289,13 +300,14 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
     int limit[NC];         // tokens that the column sees
     int least, most;       // the smallest and largest limit of the wave's real columns
 
-    __device__ __forceinline__ void start(const AttnParams &p, const Request &rq, int head, int first_row, u32x4 *room) {
+    __device__ __forceinline__ void start(const AttnParams &p, const Request &rq, const int32_t *table_row, int head, int first_row, u32x4 *room) {
         lds_q = room;
         const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
         const int cap = (int)min((int64_t)rq.len, (int64_t)p.width << p.shift);
         least = INT32_MAX;
         most = 0;
-        r = log_r = 0.f;
+        unit = scale_unit(p, table_row, head);
+        log_unit = __builtin_amdgcn_logf(unit);
         seen = 0;
         fresh = true;
 #pragma unroll
@@ -382,14 +394,15 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
             }
     }
 
-    // Moves the maximum of a column to its largest score so far; `by`: what its sum and accumulators are to be multiplied by.
-    // A column that has seen nothing keeps a maximum of 0 (its scores are -inf, its weights 0).
-    __device__ __forceinline__ void settle(const f32x4 (&s)[2], float f, int c, float &by) {
+    // Moves the maximum of a column to its largest s + log2(vs / u) so far; `by`: what its sum and accumulators are to be
+    // multiplied by.  A column that has seen nothing keeps a maximum of 0 (its scores are -inf, its weights 0).
+    __device__ __forceinline__ void settle(const f32x4 (&s)[2], float f, float add, int c, float &by) {
         float best = kNegInf;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) best = fmaxf(best, s[t][e] * f);
+        best += add;
         best = fmaxf(best, __shfl_xor(best, 16, kWave));
         best = fmaxf(best, __shfl_xor(best, 32, kWave));
         const bool any = best > kNegInf, first = !(seen & (1u << c));
@@ -438,36 +451,23 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
                     for (int e = 0; e < 4; ++e) s[c][t][e] = tok + 4 * t + e < limit[c] && held ? s[c][t][e] * f : kNegInf;
             f = 1.f;
         }
-        float by[NC], by_r = 1.f;          // what sums, and beyond that accumulators, are multiplied by
-        bool moved = false;
+        float by[NC];                      // what sums and accumulators are multiplied by
 #pragma unroll
         for (int c = 0; c < NC; ++c) by[c] = 1.f;
-        if (__builtin_expect(__any(v.scale > r), 0)) {
-            float top = fmaxf(r, v.scale);
-            if (!WIDE) {
-                top = fmaxf(top, __shfl_xor(top, 16, kWave));
-                top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            }
-            by_r = r / top;
-            r = top;
-            log_r = __builtin_amdgcn_logf(top);
-            moved = true;
-        }
-        const bool fold = !__any(held && !(v.scale >= r * kFold && v.scale >= kLeast)), early = masked || fresh || !fold;
-        const float add = fold && held ? __builtin_amdgcn_logf(v.scale) - log_r : 0.f;
-        const float back = fold && held ? r * __builtin_amdgcn_rcpf(v.scale) : 1.f, ratio = fold ? 1.f : r > 0.f ? v.scale / r : 0.f;
-        moved = moved || early;
+        const float floor = unit * 0x1p-60f, scale = fmaxf(v.scale, floor), add = __builtin_amdgcn_logf(scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(scale);
+        const bool tiny = __any(!(v.scale >= floor)), early = masked || fresh;
+        bool moved = early;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             float sum;
-            if (__builtin_expect(early, 0)) settle(s[c], f, c, by[c]);
+            if (__builtin_expect(early, 0)) settle(s[c], f, add, c, by[c]);
             w[c] = exponentials(s[c], f, add - m[c], sum);
             if (__builtin_expect(__any(sum > kMost), 0)) {
-                settle(s[c], f, c, by[c]);
+                settle(s[c], f, add, c, by[c]);
                 moved = true;
                 w[c] = exponentials(s[c], f, add - m[c], sum);
             }
-            if (__builtin_expect(!fold, 0)) w[c] = exponentials(s[c], f, -m[c], sum, ratio);
+            if (__builtin_expect(tiny, 0)) w[c] = exponentials(s[c], f, add - m[c], sum, v.scale >= floor ? 1.f : v.scale / floor);
             l[c] = fmaf(sum, back, l[c] * by[c]);
         }
         if (__builtin_expect(fresh, 0)) {
@@ -480,7 +480,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int j = 0; j < D / 16; ++j) o[c][j] *= by[c] * by_r;
+                for (int j = 0; j < D / 16; ++j) o[c][j] *= by[c];
         }
         if (__builtin_expect(nan, 0)) spread_nan(v, tok, held);
     }
@@ -549,7 +549,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         }
     }
 
-    // accumulators (already times r and joined with other waves', maximum mm, sum ll) to the result or the workspace
+    // accumulators (joined with other waves', maximum mm, sum ll) to the result or the workspace
     __device__ __forceinline__ void store(const AttnParams &p, const Request &rq, const Item &it, int64_t item, int head, int rows_per_tile,
                                           int first_in_tile, const float (&mm)[NC], const float (&ll)[NC]) {
         const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
@@ -559,7 +559,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
             if (row >= rq.rows) continue;
             if (it.chunks == 1) {
                 const int tok = row / p.group, h = head * p.group + row - tok * p.group;
-                const float by = ll[c] > 0.f || ll[c] != ll[c] ? 1.f / ll[c] : 0.f;
+                const float by = ll[c] > 0.f || ll[c] != ll[c] ? unit / ll[c] : 0.f;
                 elem *dst = static_cast<elem *>(p.out) + (int64_t)(rq.first + tok) * p.o_t + (int64_t)h * p.o_h;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -595,15 +595,14 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
     }
 };
 
-// rows behind the last request: 0, lse -inf
-template <int THREADS> __device__ __forceinline__ void clear_tail(const AttnParams &p, int head, int D) {
-    const int from = min(max(p.cu[p.n], 0), p.tokens);
-    for (int64_t x = threadIdx.x; x < (int64_t)(p.tokens - from) * p.group * D; x += THREADS) {
-        const int64_t t = from + x / (p.group * D);
-        const int h = head * p.group + (int)(x / D % p.group), d = (int)(x % D);
-        static_cast<elem *>(p.out)[t * p.o_t + h * p.o_h + d] = (elem)0.f;
-        if (p.lse && d == 0) p.lse[t * p.lse_t + h * p.lse_h] = kNegInf;
-    }
+// Rows behind the last request: 0, lse -inf.  Workgroup `part` of `parts` takes every parts-th row.
+template <int THREADS> __device__ __forceinline__ void clear_tail(const AttnParams &p, int head, int D, int part, int parts) {
+    for (int64_t t = (int64_t)min(max(p.cu[p.n], 0), p.tokens) + part; t < p.tokens; t += parts)
+        for (int x = threadIdx.x; x < p.group * D; x += THREADS) {
+            const int h = head * p.group + x / D, d = x % D;
+            static_cast<elem *>(p.out)[t * p.o_t + h * p.o_h + d] = (elem)0.f;
+            if (p.lse && d == 0) p.lse[t * p.lse_t + h * p.lse_h] = kNegInf;
+        }
 }
 
 struct AttnLaunch {

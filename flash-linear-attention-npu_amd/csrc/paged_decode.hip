@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(W * 64, NC == 2 && D == 128 ? 3 : 2) paged_dec
     __shared__ f32x4 lds_o[W / 2][D / 16 * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, i = lane & 15;
     const int head = blockIdx.x % p.heads, item = blockIdx.x / p.heads;
-    if (p.clear_tail && blockIdx.x >= gridDim.x - p.heads) clear_tail<W * 64>(p, head, D);
+    if (p.clear_tail) clear_tail<W * 64>(p, head, D, item, gridDim.x / p.heads);
     int base;
     const Item it = find_item<kRows>(p, item, false, base);
     if (!it.found) return;
@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(W * 64, NC == 2 && D == 128 ? 3 : 2) paged_dec
     pages.fill(p, row, t0, 32 * W);
     const Request rq = request_of(p, it.r);
     Walk<CODE, D, NC, WIDE, STREAM> walk;
-    walk.start(p, rq, head, it.tile * kRows, lds_q);
+    walk.start(p, rq, row, head, it.tile * kRows, lds_q);
     const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
     walk.run(p, row, pages, head, t0, 32 * W, end);
     walk.finish();
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(W * 64, NC == 2 && D == 128 ? 3 : 2) paged_dec
             const float lw = lds_ml[w][16 * c + i][1];      // 0: the wave saw no token (its maximum is -inf)
             l[c] += lw == 0.f ? 0.f : lw * exp2f(lds_ml[w][16 * c + i][0] - m[c]);
         }
-        const float by = walk.l[c] == 0.f ? 0.f : exp2f(walk.m[c] - m[c]) * walk.r;
+        const float by = walk.l[c] == 0.f ? 0.f : exp2f(walk.m[c] - m[c]);
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) walk.o[c][j] *= by;
     }
@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(64 * (WAVES > 4 ? WAVES : 4)) paged_join_kerne
     const Item it = find_item<ROWS>(p, blockIdx.x / p.heads, true, base);
     if (!it.found || it.chunks == 1) return;
     const Request rq = request_of(p, it.r);
+    const float unit = scale_unit(p, p.table + it.r * p.table_s, head);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rows = min(ROWS, rq.rows - it.tile * ROWS);
     for (int in_tile = WAVES == 1 ? blockIdx.y * 4 + wave : blockIdx.y; in_tile < rows; in_tile += gridDim.y * (WAVES == 1 ? 4 : 1)) {
         const int r = it.tile * ROWS + in_tile;
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(64 * (WAVES > 4 ? WAVES : 4)) paged_join_kerne
         }
         if (WAVES == 1 || wave == 0) {
             const int tok = r / p.group, h = head * p.group + r - tok * p.group;
-            const float by = sum.l > 0.f || sum.l != sum.l ? 1.f / sum.l : 0.f;
+            const float by = sum.l > 0.f || sum.l != sum.l ? unit / sum.l : 0.f;
             elem *dst = static_cast<elem *>(p.out) + (int64_t)(rq.first + tok) * p.o_t + (int64_t)h * p.o_h;
 #pragma unroll
             for (int x = 0; x < V; ++x) dst[lane * V + x] = (elem)(sum.o[x] * by);

@@ -12,9 +12,9 @@ __global__ void __launch_bounds__(64, 2) paged_prefill_kernel(const AttnParams p
     constexpr int kRows = 16 * NC;
     __shared__ u32x4 lds_q[NC * (D / 32) * 64];
     const int head = blockIdx.x % p.heads;
-    if (p.clear_tail && blockIdx.x < p.heads) clear_tail<64>(p, head, D);
     int base;
     const int item = (gridDim.x - 1 - blockIdx.x) / p.heads;      // long rows of a request first
+    if (p.clear_tail) clear_tail<64>(p, head, D, item, gridDim.x / p.heads);
     const Item it = find_item<kRows>(p, item, false, base);
     if (!it.found) return;
     const int64_t from = (int64_t)it.chunk * it.units * kUnit;
@@ -24,14 +24,10 @@ __global__ void __launch_bounds__(64, 2) paged_prefill_kernel(const AttnParams p
     pages.fill(p, row, t0, 32);
     const Request rq = request_of(p, it.r);
     Walk<CODE, D, NC, WIDE, false> walk;
-    walk.start(p, rq, head, it.tile * kRows, lds_q);
+    walk.start(p, rq, row, head, it.tile * kRows, lds_q);
     const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
     walk.run(p, row, pages, head, t0, 32, end);
     walk.finish();
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) walk.o[c][j] *= walk.r;
     walk.store(p, rq, it, item, head, kRows, 0, walk.m, walk.l);
 }
 

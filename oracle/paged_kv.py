@@ -96,15 +96,17 @@ def append(x, codes, scales, slots, dtype):
         t += n
 
 
-def attention(q, key_codes, value_codes, key_scales, value_scales, table, lens, cu, scale, rows=None):
-    """float64 (out, lse, spread, reach) for codes given as float64 [P,H,page,D].  ``spread``: the weighted mean of |v|, and
-    ``reach``: the largest scale * sum |q||k| of a row, which bound the effect of relative errors of the weights and of the
-    scores.  ``rows``: cu as a list; None for one row each."""
+def attention(q, key_codes, value_codes, key_scales, value_scales, table, lens, cu, scale):
+    """float64 (out, lse, spread, reach, peak) for codes given as float64 [P,H,page,D].  ``spread``: the weighted mean of |v|,
+    ``reach``: the largest scale * sum |q||k| of a row, and ``peak``: the largest p * value scale of a row: they bound the
+    effect of relative errors of the weights, of the scores, and of absolute errors of the weights.  ``cu`` None: one row
+    for each request."""
     tokens, heads, d = q.shape
     pool, kv_heads, page, _ = key_codes.shape
     group = heads // kv_heads
     out, spread = torch.zeros(tokens, heads, d, dtype=torch.float64), torch.zeros(tokens, heads, d, dtype=torch.float64)
     lse, reach = torch.full((tokens, heads), -math.inf, dtype=torch.float64), torch.zeros(tokens, heads, dtype=torch.float64)
+    peak = torch.zeros(tokens, heads, dtype=torch.float64)
     cu = list(range(len(lens) + 1)) if cu is None else [int(c) for c in cu]
     for r, length in enumerate(int(n) for n in lens):
         blocks = [int(b) for b in table[r]]
@@ -128,5 +130,6 @@ def attention(q, key_codes, value_codes, key_scales, value_scales, table, lens, 
                 sl = (cu[r] + j, slice(h * group, (h + 1) * group))
                 out[sl], spread[sl] = p @ v[:n], p @ v[:n].abs()
                 lse[sl] = torch.logsumexp(s, -1)
+                peak[sl] = (p * value_scales[block[:n], h].double().abs()).amax(-1)
                 reach[sl] = (qs.abs() @ k[:n].abs().t()).amax(-1) * abs(scale)
-    return out, lse, spread, reach
+    return out, lse, spread, reach, peak

@@ -288,7 +288,7 @@ def test_oracle_attention_is_softmax_attention():
     ks, vs = torch.rand(4, 2, generator=gen), torch.rand(4, 2, generator=gen)
     q = torch.randn(5, 4, 64, generator=gen)
     table = torch.tensor([[2, 0, 3]])
-    out, lse, spread, _ = ref.attention(q, kc, vc, ks, vs, table, [37], [0, 5], 0.125)
+    out, lse, spread, *_ = ref.attention(q, kc, vc, ks, vs, table, [37], [0, 5], 0.125)
     k = (kc * ks.double()[..., None, None])[[2, 0, 3]].transpose(1, 2).flatten(0, 1)[:37].transpose(0, 1).repeat_interleave(2, 0)
     v = (vc * vs.double()[..., None, None])[[2, 0, 3]].transpose(1, 2).flatten(0, 1)[:37].transpose(0, 1).repeat_interleave(2, 0)
     mask = torch.arange(37) <= torch.arange(32, 37)[:, None]

@@ -7,8 +7,8 @@ Bounds (eps = torch.finfo(type).eps; a rounding is off by at most eps / 2 of the
   |a| + |b| <= 2^-21 (|a| + |b|) in all.
 * attention: one rounding to the output type.  Every weight carries 2^-12 (fp16) and the error of its score: a sum of D
   products in fp32, at most (D + 8) * 2^-24 of sum |q||k| * scale, twice (weight and normalisation).  These are relative
-  errors of weights, so they count for sum p|v| ("spread").  A weight below 2^-14 is off by at most 2^-25 of
-  the largest scale times the largest code, for each token.  lse: the score error, and 2^-21 of its value.
+  errors of weights, so they count for sum p|v| ("spread").  A weight below 2^-14 is off by at most 2^-25 of the
+  row's largest p * value scale ("peak") times the largest code, for each token.  lse: the score error, and 2^-21 of its value.
 """
 import math
 import random
@@ -262,10 +262,10 @@ def check_attention(dev, q, caches, table, lens, cu, scale, *, got=None, **kw):
     if got is None:
         got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, table.to(dev), i32(lens), None if cu is None else i32(cu), scale=scale, return_lse=True, **kw)
     out, lse = (t.cpu().double() for t in got)
-    want, want_lse, spread, reach = ref.attention(q, codes_of(kc), codes_of(vc), ks.cpu(), vs.cpu(), table, lens, cu, scale)
+    want, want_lse, spread, reach, peak = ref.attention(q, codes_of(kc), codes_of(vc), ks.cpu(), vs.cpu(), table, lens, cu, scale)
     d = q.shape[-1]
     score = (d + 8) * 2.0 ** -24 * reach
-    top = float(vs.max()) * ref.LARGEST[kc.dtype]
+    top = peak[..., None] * ref.LARGEST[kc.dtype]
     bound = want.abs() * torch.finfo(q.dtype).eps / 2 * 1.01 + spread * (2.0 ** -12 * 1.01 + 2 * score[..., None]) + max(lens) * 2.0 ** -25 * top + torch.finfo(q.dtype).tiny
     assert torch.equal(out.isnan(), want.isnan())
     error = torch.where(want.isnan(), 0.0, (out - want).abs())
@@ -408,6 +408,11 @@ def test_scales_of_very_different_sizes(dev, new):
     table = make_table(rng, lens, page, 21, pool)
     q = torch.randn(2 * new, heads, dim, generator=gen).to(BF)
     check_attention(dev, q, (kc, vc, ks, vs), table, lens, [0, new, 2 * new], dim ** -0.5)
+    # one request whose rows look at pages with tiny values next to pages with large ones that they all but ignore
+    kc.copy_(torch.where(torch.rand(pool, 1, 1, 1, generator=gen) < 0.5, 1.0, -1.0).expand(pool, kv_heads, page, dim).to(E4M3))
+    ks.fill_(1.0)
+    vs.copy_(torch.where(codes_of(kc)[:, 0, 0, :1] > 0, 2.0 ** -30, 2.0 ** 10).expand(pool, kv_heads).float())
+    check_attention(dev, torch.full((2 * new, heads, dim), 0.5).to(BF), (kc, vc, ks, vs), table, lens, [0, new, 2 * new], 0.5)
     vs.fill_(2.0 ** -120)                  # fp32 holds it, the result type bf16 as well
     check_attention(dev, q, (kc, vc, ks, vs), table, lens, [0, new, 2 * new], dim ** -0.5)
     vs.zero_()
