@@ -477,6 +477,173 @@ def test_cache_beyond_32_bit_offsets(dev):
     check_attention(dev, q, small, torch.tensor([[0, 1, 2]], dtype=torch.int32), lens, None, dim ** -0.5, got=got)
 
 
+# Tables that name more than 2048 tokens split the keys over workgroups, whatever the lengths are.
+WIDE = 5000
+
+
+def widen(table, page):
+    more = torch.full((table.shape[0], -(-WIDE // page)), -1, dtype=torch.int32)
+    return torch.cat([table, more], 1)
+
+
+@pytest.mark.parametrize("page,heads,kv_heads,dim,dtype,code", DECODE + [(32, 80, 1, 64, BF, E4M3)])
+def test_wide_tables(dev, page, heads, kv_heads, dim, dtype, code):
+    rng, gen = random.Random(page + heads), torch.Generator().manual_seed(heads * dim + 1)
+    lens = [1, 0, 17, 700, 33, 1300, 2, 511, 513]
+    pool = sum(-(-n // page) for n in lens) + 5
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, code, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, code, dev)
+    table = widen(make_table(rng, lens, page, max(-(-n // page) for n in lens), pool), page)
+    table[5, 3] = pool + 4                                      # a page that is not there
+    q = torch.randn(len(lens), heads, dim, generator=gen).to(dtype)
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, None, dim ** -0.5)
+    cu = [0, 1, 1, 8, 11, 11, 20, 22, 23, 40]
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(dtype)
+    for hint in (17, 3, None):
+        check_attention(dev, q, (kc, vc, ks, vs), table, lens, cu, dim ** -0.5, max_query_len=hint)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("n,most,new", [(150, 90, 1), (200, 400, 3), (130, 60, 25)])
+def test_many_requests(dev, n, most, new, wide):
+    """More requests than a wave has lanes; requests without rows and without tokens among them."""
+    rng, gen = random.Random(n), torch.Generator().manual_seed(n)
+    page, heads, kv_heads, dim = 16, 6, 2, 64
+    rows = [rng.choice([0, 1, rng.randint(1, new)]) if new > 1 else 1 for _ in range(n)]
+    lens = [rng.choice([r, r + rng.randint(0, most)]) for r in rows]
+    cu = [0]
+    for r in rows:
+        cu.append(cu[-1] + r)
+    pool = sum(-(-m // page) for m in lens) + 3
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    table = make_table(rng, lens, page, max(-(-m // page) for m in lens), pool)
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(F16)
+    check_attention(dev, q, (kc, vc, ks, vs), widen(table, page) if wide else table, lens, None if new == 1 else cu, dim ** -0.5, max_query_len=new)
+
+
+@pytest.mark.parametrize("new", [1, 5, 80])
+def test_what_is_not_seen_may_hold_anything_in_wide_tables(dev, new):
+    rng, gen = random.Random(5), torch.Generator().manual_seed(5)
+    page, heads, kv_heads, dim, lens = 16, 8, 2, 128, [new + 5, new + 900, new, new + 300]
+    pool = sum(-(-n // page) for n in lens) + 4
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    table = widen(make_table(rng, lens, page, max(-(-n // page) for n in lens), pool), page)
+    nobody = sorted(set(range(pool)) - set(table[table >= 0].tolist()))
+    safe = [c.view(torch.uint8).clone().view(E4M3) for c in (kc, vc)] + [ks.clone(), vs.clone()]
+    for c in (kc, vc):
+        c.view(torch.uint8)[nobody] = 0x7f
+        for r, n in enumerate(lens):
+            if n % page:
+                c.view(torch.uint8)[int(table[r, (n - 1) // page]), :, n % page:] = 0xff
+    ks[nobody], vs[nobody] = math.nan, math.inf
+    bad = table.clone()
+    bad[table < 0] = nobody[0]
+    cu = [new * r for r in range(len(lens) + 1)]
+    q = torch.randn(cu[-1], heads, dim, generator=gen).to(BF)
+    from fla_hip import ops
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, bad.to(dev), i32(lens), i32(cu), max_query_len=new, return_lse=True)
+    check_attention(dev, q, safe, table, lens, cu, dim ** -0.5, got=got)
+
+
+@pytest.mark.parametrize("code,dtype,page", [(E4M3, BF, 64), (INT8, F16, 16)])
+def test_prefill_that_fills_the_chip(dev, code, dtype, page):
+    """Enough tiles that keys are not split; against the formula in float64 on the GPU, a head at a time.  Padded rows."""
+    from fla_hip import ops
+    gen, rng = torch.Generator().manual_seed(3), random.Random(3)
+    heads, kv_heads, dim, lens, rows, pad = 64, 64, 64, [2100, 700], [2000, 333], 30
+    cu = [0, 2000, 2333]
+    pool = sum(-(-n // page) for n in lens) + 2
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, code, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, code, dev)
+    table = make_table(rng, lens, page, -(-lens[0] // page), pool).to(dev)
+    q = torch.randn(cu[-1] + pad, heads, dim, generator=gen).to(dtype).to(dev)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    out, lse = ops.paged_kv_attention(q, kc, vc, ks, vs, table, i32(lens), i32(cu), max_query_len=2000, return_lse=True)
+    assert bool((out[cu[-1]:] == 0).all()) and bool((lse[cu[-1]:] == -math.inf).all())
+    values = lambda c, s, blocks, h: ((c[blocks, h].double() if code == INT8 else c.view(torch.uint8)[blocks, h].view(E4M3).float().double()) * s[blocks, h].double()[:, None, None]).flatten(0, 1)
+    for r, n in enumerate(lens):
+        blocks = table[r, :-(-n // page)].long()
+        seen = torch.arange(n, device=dev) <= torch.arange(n - rows[r], n, device=dev)[:, None]
+        for h in range(0, heads, 5):
+            k, v = (values(c, s, blocks, h)[:n] for c, s in ((kc, ks), (vc, vs)))
+            x = q[cu[r]:cu[r + 1], h].double()
+            score = torch.where(seen, (x @ k.t()) * dim ** -0.5, -math.inf)
+            p = torch.softmax(score, -1)
+            want, spread = p @ v, p @ v.abs()
+            err = (dim + 8) * 2.0 ** -24 * ((x.abs() @ k.abs().t()) * dim ** -0.5).amax(-1)
+            peak = (p * vs[blocks, h].double().repeat_interleave(page)[:n]).amax(-1)[:, None] * ref.LARGEST[code]
+            bound = want.abs() * torch.finfo(dtype).eps / 2 * 1.01 + spread * (2.0 ** -12 * 1.01 + 2 * err[:, None]) + n * 2.0 ** -25 * peak + torch.finfo(dtype).tiny
+            assert bool(((out[cu[r]:cu[r + 1], h].double() - want).abs() <= bound).all()), (r, h)
+            assert bool(((lse[cu[r]:cu[r + 1], h].double() - score.logsumexp(-1)).abs() <= err + 2.0 ** -21 * (1 + score.logsumexp(-1).abs())).all()), (r, h)
+
+
+def test_split_attention_replays_from_a_graph(dev):
+    """Lengths, tables and rows change between replays; eager calls with other sizes use workspaces in between."""
+    from fla_hip import ops
+    gen, rng = torch.Generator().manual_seed(8), random.Random(8)
+    page, heads, kv_heads, dim, n, T = 64, 8, 2, 128, 3, 7
+    pool, width = 200, -(-WIDE // page)
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    buf = dict(q=torch.zeros(T, heads, dim, dtype=BF, device=dev), table=torch.zeros(n, width, dtype=torch.int32, device=dev),
+               lens=torch.ones(n, dtype=torch.int32, device=dev), cu=torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=dev))
+    call = lambda: ops.paged_kv_attention(buf["q"], kc, vc, ks, vs, buf["table"], buf["lens"], buf["cu"], max_query_len=4, return_lse=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for g in graphs:                                             # two graphs of the same call, replayed in turn
+        with torch.cuda.graph(g):
+            outs.append(call())
+    for trial in range(4):
+        lens = [rng.choice([1, 70, 3000, 4900]) for _ in range(n)]
+        cu = [0, 1, 1 + trial, 4 + trial - (trial > 2)]
+        table = make_table(rng, lens, page, width, pool)
+        lens = [max(m, b - a) for m, a, b in zip(lens, cu, cu[1:])]
+        q = torch.randn(T, heads, dim, generator=gen).to(BF)
+        for name, v in (("q", q), ("table", table), ("lens", torch.tensor(lens)), ("cu", torch.tensor(cu))):
+            buf[name].copy_(v)
+        eager = [t.clone() for t in call()]
+        ops.paged_kv_attention(buf["q"][:n], kc, vc, ks, vs, buf["table"], buf["lens"])
+        torch.cuda.synchronize()
+        for g, out in zip(graphs, outs):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1]), trial
+        check_attention(dev, q[:cu[-1]], (kc, vc, ks, vs), table, lens, cu, dim ** -0.5, got=tuple(t[:cu[-1]] for t in eager))
+
+
+def test_append_of_many_rows(dev):
+    """Workgroups that look for first rows among 32: runs that begin and end anywhere, pages longer than what a wave sees at
+    once, skipped rows, a run as long as its page, the last row alone."""
+    from fla_hip import ops
+    rng, gen = random.Random(2), torch.Generator().manual_seed(2)
+    page, heads, dim, pool = 128, 8, 64, 700
+    ids, slots = list(range(pool)), []
+    rng.shuffle(ids)
+    while len(slots) < 33000 and ids:
+        if rng.random() < 0.1:
+            slots += [-1] * rng.randint(1, 40)
+            continue
+        off = rng.choice([0, 0, 1, rng.randint(0, page - 1)])
+        n = rng.choice([1, 2, page - off, page - off, rng.randint(1, page - off)])
+        slots += range(ids[-1] * page + off, ids.pop() * page + off + n)
+    assert len(slots) * heads * 2 >= 8192 * 32
+    kc, ks = random_cache(gen, pool, heads, page, dim, INT8, dev)
+    vc, vs = random_cache(gen, pool, heads, page, dim, INT8, dev)
+    x = torch.randn(len(slots), heads, dim, generator=gen).to(BF)
+    want, scale = codes_of(kc), ks.cpu().double()
+    ops.paged_kv_append(x.to(dev), x.flip(0).to(dev), kc, vc, ks, vs, torch.tensor(slots, device=dev))
+    ref.append(x, want, scale, slots, INT8)
+    assert torch.equal(ks.cpu().double(), scale) and torch.equal(codes_of(kc), want)
+
+
 # ---- together --------------------------------------------------------------------------------------------------------
 
 def serve(dev, steps, code, capture, side_stream=False):
