@@ -183,7 +183,10 @@ template <bool WIDE> struct PageWindow {
         entries = at < p.width ? row[at] : -1;
     }
     __device__ __forceinline__ Place<WIDE> get(const AttnParams &p, const int32_t *row, int t0, int stride, int step, int most) {
-        if (step && (step & (WIDE ? 63 : 31)) == 0) fill(p, row, t0, stride);
+        if (__builtin_expect(step && (step & (WIDE ? 63 : 31)) == 0, 0)) {
+            fill(p, row, t0, stride);
+            asm volatile("" : "+v"(entries));      // waited for here: behind the branch every step would wait for all its loads
+        }
         const int k = step & (WIDE ? 63 : 31);
         int page;
         if (WIDE) page = __builtin_amdgcn_readlane(entries, k);
@@ -521,18 +524,17 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
     __device__ __forceinline__ void accumulate(const ValueCodes<D, WIDE, STREAM> &v, const f16x8 (&w)[NC]) {   // O^T += V^T P^T
 #pragma unroll
         for (int x = 0; x < D / 64; ++x) {
-            unsigned wide[8][2];
+            unsigned pair[4][2];                      // bytes of two tokens side by side, channel by channel
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                wide[e][0] = widen2<CODE, f16, 0>(v.c[e][x]);
-                wide[e][1] = widen2<CODE, f16, 1>(v.c[e][x]);
+            for (int e = 0; e < 4; ++e) {
+                pair[e][0] = __builtin_amdgcn_perm(v.c[2 * e + 1][x], v.c[2 * e][x], 0x05010400u);
+                pair[e][1] = __builtin_amdgcn_perm(v.c[2 * e + 1][x], v.c[2 * e][x], 0x07030602u);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 u32x4 a;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    a[e] = __builtin_amdgcn_perm(wide[2 * e + 1][j >> 1], wide[2 * e][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+                for (int e = 0; e < 4; ++e) a[e] = (j & 1) ? widen2<CODE, f16, 1>(pair[e][j >> 1]) : widen2<CODE, f16, 0>(pair[e][j >> 1]);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) o[c][4 * x + j] = mfma16x32(__builtin_bit_cast(f16x8, a), w[c], o[c][4 * x + j]);
             }

@@ -39,27 +39,32 @@ class _Call:
     def __init__(self, anchor, name: str):
         _runtime.ensure_gpu_tensor(anchor, name)
         self.device = anchor.device
+        self.index = anchor.get_device()
 
     def tensor(self, t, name: str):
         if t is None:
             return None
         try:
-            device, dtype, shape, stride, ptr = t.device, t.dtype, t.shape, t.stride(), t.data_ptr()
-        except AttributeError:
-            raise TypeError(f"{name} must be a torch.Tensor, got {type(t)!r}.") from None
-        if device != self.device:
-            _runtime.ensure_gpu_tensor(t, name)
-            raise ValueError(f"{name} must be on {self.device}, got {device}; one call cannot mix tensors from different devices.")
-        code = _CODE_OF.get(dtype)
+            if t.get_device() == self.index:
+                shape = t.shape
+                n = len(shape)
+                return _FLA_TENSOR[n].pack(t.data_ptr(), _CODE_OF[t.dtype], n, *shape, *t.stride())
+        except (AttributeError, KeyError, IndexError):
+            pass
+        return self._checked(t, name)
+
+    def _checked(self, t, name: str):
+        """What is wrong with ``t``; or a type seen for the first time."""
+        _runtime.ensure_gpu_tensor(t, name)
+        if t.device != self.device:
+            raise ValueError(f"{name} must be on {self.device}, got {t.device}; one call cannot mix tensors from different devices.")
+        if t.dim() > _runtime.FLA_MAX_DIMS:
+            raise ValueError(f"{name} has rank {t.dim()} > {_runtime.FLA_MAX_DIMS}.")
+        code = _CODES.get(str(t.dtype))
         if code is None:
-            code = _CODES.get(str(dtype))
-            if code is None:
-                raise TypeError(f"fla_hip: unsupported tensor dtype {dtype}.")
-            _CODE_OF[dtype] = code
-        n = len(shape)
-        if n > _runtime.FLA_MAX_DIMS:
-            raise ValueError(f"{name} has rank {n} > {_runtime.FLA_MAX_DIMS}.")
-        return _FLA_TENSOR[n].pack(ptr, code, n, *shape, *stride)
+            raise TypeError(f"fla_hip: {name} has unsupported tensor dtype {t.dtype}.")
+        _CODE_OF[t.dtype] = code
+        return self.tensor(t, name)
 
     def run(self, name: str, *args):
         """``fla_<name>(<operands>, stream)`` on the current stream of the call's device."""
