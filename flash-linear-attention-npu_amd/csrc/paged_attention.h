@@ -353,26 +353,72 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         ValueCodes<D, WIDE, STREAM> v;
         Place<WIDE> at = pages.get(p, row, t0, stride, 0, most);
         k.load(p, head, t0, at, off);
-        if (STREAM) v.load(p, head, t0, at, off);
-        for (int step = 1;; ++step) {
-            const int t1 = t0 + stride;
-            const bool go = t1 < end;
-            f32x4 s[NC][2];
-            Place<WIDE> next = at;
-            if (!STREAM) v.load(p, head, t0, at, off);
-            scores(k, s);
-            const float f = k.scale * p.scale2;
-            if (go) next = pages.get(p, row, t1, stride, step, most);
-            if (STREAM && go) k.load(p, head, t1, next, off);
-            f16x8 w[NC];
-            weigh(s, f, v, at.held, t0, w);
-            if (!STREAM && go) k.load(p, head, t1, next, off);
-            accumulate(v, w);
-            if (!go) break;
-            if (STREAM) v.load(p, head, t1, next, off);
-            at = next;
-            t0 = t1;
+        if constexpr (STREAM) {
+            v.load(p, head, t0, at, off);
+            for (int step = 1;; ++step) {
+                const int t1 = t0 + stride;
+                const bool go = t1 < end;
+                f32x4 s[NC][2];
+                Place<WIDE> next = at;
+                scores(k, s);
+                const float f = k.scale * p.scale2;
+                if (go) {
+                    next = pages.get(p, row, t1, stride, step, most);
+                    k.load(p, head, t1, next, off);
+                }
+                f16x8 w[NC];
+                weigh(s, f, v, at.held, t0, w);
+                accumulate(v, w);
+                if (!go) break;
+                v.load(p, head, t1, next, off);
+                at = next;
+                t0 = t1;
+            }
+        } else {
+            // Steps that every column sees whole, and that move no maximum, have a loop of their own: with the code for the
+            // others in it, the compiler keeps the accumulators in memory for part of it.
+            for (int step = 1; t0 < end;) {
+                while (t0 < end && t0 + 32 <= least && !fresh) {
+                    v.load(p, head, t0, at, off);
+                    f32x4 s[NC][2];
+                    scores(k, s);
+                    const float f = k.scale * p.scale2, floor = unit * 0x1p-60f;
+                    const float add = __builtin_amdgcn_logf(v.scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(v.scale);
+                    f16x8 w[NC];
+                    float sum[NC], top = 0.f;
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        w[c] = exponentials(s[c], f, add - m[c], sum[c]);
+                        top = fmaxf(top, sum[c]);
+                    }
+                    if (__builtin_expect(__any(top > kMost || !at.held || !(v.scale >= floor)), 0)) break;
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) l[c] = fmaf(sum[c], back, l[c]);
+                    advance(p, row, pages, head, t0, stride, end, step, at, k, off);
+                    accumulate(v, w);
+                }
+                if (t0 >= end) break;
+                v.load(p, head, t0, at, off);
+                f32x4 s[NC][2];
+                scores(k, s);
+                f16x8 w[NC];
+                fresh = true;                  // every maximum settles
+                weigh(s, k.scale * p.scale2, v, at.held, t0, w);
+                advance(p, row, pages, head, t0, stride, end, step, at, k, off);
+                accumulate(v, w);
+            }
         }
+    }
+
+    // to the next step, whose keys are loaded if there is one
+    __device__ __forceinline__ void advance(const AttnParams &p, const int32_t *row, PageWindow<WIDE> &pages, int head, int &t0, int stride, int end,
+                                            int &step, Place<WIDE> &at, KeyCodes<D, WIDE, STREAM> &k, const LaneOffsets &off) {
+        t0 += stride;
+        if (t0 < end) {
+            at = pages.get(p, row, t0, stride, step, most);
+            k.load(p, head, t0, at, off);
+        }
+        ++step;
     }
 
     __device__ __forceinline__ void scores(const KeyCodes<D, WIDE, STREAM> &k, f32x4 (&s)[NC][2]) {
