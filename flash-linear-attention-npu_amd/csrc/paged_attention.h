@@ -426,21 +426,24 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));        // the reads below stay in the loop: hoisted, the queries would take registers again
+        u32x4 b[2][NC];                                  // the next queries are read while these are used
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h)
+        for (int c = 0; c < NC; ++c) b[0][c] = kQueriesInLds ? lds_q[c * (D / 32) * 64 + lane] : q[kQueriesInLds ? 0 : c][0];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                u32x4 b[NC];
+        for (int i = 0; i < D / 32; ++i) {
+            if (i + 1 < D / 32) {
 #pragma unroll
-                for (int c = 0; c < NC; ++c) b[c] = kQueriesInLds ? lds_q[(c * (D / 32) + 2 * h + half) * 64 + lane] : q[kQueriesInLds ? 0 : c][2 * h + half];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const u32x4 a = {widen2<CODE, elem, 0>(k.c[t][h][2 * half]), widen2<CODE, elem, 1>(k.c[t][h][2 * half]),
-                                     widen2<CODE, elem, 0>(k.c[t][h][2 * half + 1]), widen2<CODE, elem, 1>(k.c[t][h][2 * half + 1])};
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) s[c][t] = mfma16x32(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b[c]), s[c][t]);
-                }
+                for (int c = 0; c < NC; ++c) b[(i + 1) & 1][c] = kQueriesInLds ? lds_q[(c * (D / 32) + i + 1) * 64 + lane] : q[kQueriesInLds ? 0 : c][i + 1];
             }
+            if (kQueriesInLds) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const u32x4 a = {widen2<CODE, elem, 0>(k.c[t][i >> 1][2 * (i & 1)]), widen2<CODE, elem, 1>(k.c[t][i >> 1][2 * (i & 1)]),
+                                 widen2<CODE, elem, 0>(k.c[t][i >> 1][2 * (i & 1) + 1]), widen2<CODE, elem, 1>(k.c[t][i >> 1][2 * (i & 1) + 1])};
+#pragma unroll
+                for (int c = 0; c < NC; ++c) s[c][t] = mfma16x32(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b[i & 1][c]), s[c][t]);
+            }
+        }
     }
 
     // Moves the maximum of a column to its largest s + log2(vs / u) so far; `by`: what its sum and accumulators are to be

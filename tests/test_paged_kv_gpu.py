@@ -437,6 +437,28 @@ def test_peaked_and_far_scores(dev):
     check_attention(dev, -q, (kc, vc, ks, vs), table, lens, None, 1.0)
 
 
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("new", [1, 20, 90])
+def test_scores_that_jump_up_along_the_text(dev, new, wide):
+    """Scores rise by 2 to 400 (in log2) from one step to the next, in steps that every row sees whole: maxima move by little
+    (weights still fit fp16) and by much (they do not)."""
+    rng, gen = random.Random(10), torch.Generator().manual_seed(10)
+    page, heads, kv_heads, dim, n = 32, 4, 1, 64, 700
+    kc, ks = random_cache(gen, 60, kv_heads, page, dim, INT8, dev)
+    vc, vs = random_cache(gen, 60, kv_heads, page, dim, INT8, dev)
+    lens = [n + new, n + new - 100]
+    table = make_table(rng, lens, page, -(-max(lens) // page), 60)
+    ks.fill_(2.0 ** -4)
+    level = [1, 2, 3, 8, 9, 20, 21, 22, 50, 51, 52, 53, 100, 101, 126, 127]
+    for r in range(2):
+        for t in range(lens[r]):
+            kc[int(table[r, t // page]), 0, t % page, 0] = level[min(t // 40, 15)] if t % 40 >= 33 else 0
+    for weight in (2.0, 40.0, -40.0):                      # channel 0 of the queries: log2 of the weights rises by up to 400
+        q = torch.randn(2 * new, heads, dim, generator=gen) * 0.1
+        q[:, :, 0] = weight
+        check_attention(dev, q.to(BF), (kc, vc, ks, vs), widen(table, page) if wide else table, lens, [0, new, 2 * new], 1.0, max_query_len=new)
+
+
 def test_given_out_keeps_the_rows_behind_the_last_request(dev):
     from fla_hip import ops
     rng, gen = random.Random(9), torch.Generator().manual_seed(9)
