@@ -206,13 +206,17 @@ struct LaneOffsets {
     unsigned k, v;
 };
 
-// STREAM: loads that do not stay in the caches.
-template <bool STREAM, typename V> __device__ __forceinline__ V load_codes(const uint8_t *p) {
-    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
+// How a walk loads codes: kAhead (decode, memory far away): the next step's keys as soon as this step's are consumed, its
+// values likewise; kAheadOnce: the same past the caches, for codes that nobody reads again.  kLate (prefill, keys in L2):
+// values ahead of the first product and keys ahead of the second, which leaves 32 registers more.
+enum Loads { kLate, kAhead, kAheadOnce };
+
+template <Loads L, typename V> __device__ __forceinline__ V load_codes(const uint8_t *p) {
+    if constexpr (L == kAheadOnce) return __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
     else return *reinterpret_cast<const V *>(p);
 }
 
-template <int D, bool WIDE, bool STREAM> struct KeyCodes {
+template <int D, bool WIDE, Loads L> struct KeyCodes {
     u32x4 c[2][D / 64];
     float scale;
     __device__ __forceinline__ void load(const AttnParams &p, int head, int t0, const Place<WIDE> &pl, const LaneOffsets &off) {
@@ -224,7 +228,7 @@ template <int D, bool WIDE, bool STREAM> struct KeyCodes {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) c[t][h] = load_codes<STREAM, u32x4>(at + (int64_t)(4 * t) * p.kc_t + 64 * h + off.k);
+                for (int h = 0; h < D / 64; ++h) c[t][h] = load_codes<L, u32x4>(at + (int64_t)(4 * t) * p.kc_t + 64 * h + off.k);
         } else {
             // the rows of this lane are those of lane group i / 4, whose page sits in lane 16 (i / 4)
             const int kg = i >> 2, page = __shfl(pl.page, kg * 16, kWave);
@@ -232,12 +236,12 @@ template <int D, bool WIDE, bool STREAM> struct KeyCodes {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) c[t][h] = load_codes<STREAM, u32x4>(at + 4 * t * p.kc_t + 64 * h);
+                for (int h = 0; h < D / 64; ++h) c[t][h] = load_codes<L, u32x4>(at + 4 * t * p.kc_t + 64 * h);
         }
     }
 };
 
-template <int D, bool WIDE, bool STREAM> struct ValueCodes {
+template <int D, bool WIDE, Loads L> struct ValueCodes {
     unsigned c[8][D / 64];
     float scale;
     __device__ __forceinline__ void load(const AttnParams &p, int head, int t0, const Place<WIDE> &pl, const LaneOffsets &off) {
@@ -251,9 +255,9 @@ template <int D, bool WIDE, bool STREAM> struct ValueCodes {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint8_t *from = WIDE ? at + (int64_t)e * p.vc_t + off.v : at + e * p.vc_t;
-            if constexpr (D == 64) c[e][0] = load_codes<STREAM, unsigned>(from);
+            if constexpr (D == 64) c[e][0] = load_codes<L, unsigned>(from);
             else {
-                const VV x = load_codes<STREAM, VV>(from);
+                const VV x = load_codes<L, VV>(from);
 #pragma unroll
                 for (int w = 0; w < D / 64; ++w) c[e][w] = x[w];
             }
@@ -286,10 +290,8 @@ __device__ __forceinline__ float scale_unit(const AttnParams &p, const int32_t *
 //  - weights are rounded to fp16 with 11 bits: a bf16 weight would add an error as large as the rounding of the result.
 //  - the maximum moves only when the eight weights of a lane sum to more than 2^11 (fp16 holds 2^16), which the sum that is
 //    needed anyway tells, so most steps take no maximum, exchange nothing between lanes and rescale nothing.
-// STREAM (decode, memory far away): the next step's keys are loaded as soon as this step's are consumed, its values likewise.
-// Else (prefill, keys in L2): values are loaded ahead of the first product and keys ahead of the second, which leaves 32
-// registers more, and room for two waves on a SIMD.  Sums and statistics are fp32.
-template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
+// Sums and statistics are fp32.
+template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
     typedef elemx8 T8;
     static constexpr float kMost = 0x1p11f;
     f32x4 o[NC][D / 16];   // o[c][j][e] of lane (g, i): channel D/16 (4 g + e) + j of query row 16 c + i, in units of u 2^m
@@ -349,11 +351,11 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         LaneOffsets off;
         off.k = (unsigned)(8 * (i >> 2) + (i & 3)) * (unsigned)p.kc_t + 16 * g;
         off.v = (unsigned)(8 * g) * (unsigned)p.vc_t + i * (D / 16);
-        KeyCodes<D, WIDE, STREAM> k;
-        ValueCodes<D, WIDE, STREAM> v;
-        Place<WIDE> at = pages.get(p, row, t0, stride, 0, most);
-        k.load(p, head, t0, at, off);
-        if constexpr (STREAM) {
+        if constexpr (L != kLate) {
+            KeyCodes<D, WIDE, L> k;
+            ValueCodes<D, WIDE, L> v;
+            Place<WIDE> at = pages.get(p, row, t0, stride, 0, most);
+            k.load(p, head, t0, at, off);
             v.load(p, head, t0, at, off);
             for (int step = 1;; ++step) {
                 const int t1 = t0 + stride;
@@ -375,6 +377,10 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
                 t0 = t1;
             }
         } else {
+            KeyCodes<D, WIDE, L> k;
+            ValueCodes<D, WIDE, L> v;
+            Place<WIDE> at = pages.get(p, row, t0, stride, 0, most);
+            k.load(p, head, t0, at, off);
             // Steps that every column sees whole, and that move no maximum, have a loop of their own: with the code for the
             // others in it, the compiler keeps the accumulators in memory for part of it.
             for (int step = 1; t0 < end;) {
@@ -412,7 +418,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
 
     // to the next step, whose keys are loaded if there is one
     __device__ __forceinline__ void advance(const AttnParams &p, const int32_t *row, PageWindow<WIDE> &pages, int head, int &t0, int stride, int end,
-                                            int &step, Place<WIDE> &at, KeyCodes<D, WIDE, STREAM> &k, const LaneOffsets &off) {
+                                            int &step, Place<WIDE> &at, KeyCodes<D, WIDE, L> &k, const LaneOffsets &off) {
         t0 += stride;
         if (t0 < end) {
             at = pages.get(p, row, t0, stride, step, most);
@@ -421,7 +427,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         ++step;
     }
 
-    __device__ __forceinline__ void scores(const KeyCodes<D, WIDE, STREAM> &k, f32x4 (&s)[NC][2]) {
+    __device__ __forceinline__ void scores(const KeyCodes<D, WIDE, L> &k, f32x4 (&s)[NC][2]) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4{0.f, 0.f, 0.f, 0.f};
         int lane = threadIdx.x & 63;
@@ -480,7 +486,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
         return __builtin_bit_cast(f16x8, packed);
     }
 
-    __device__ __forceinline__ void weigh(f32x4 (&s)[NC][2], float f, ValueCodes<D, WIDE, STREAM> &v, bool held, int t0, f16x8 (&w)[NC]) {
+    __device__ __forceinline__ void weigh(f32x4 (&s)[NC][2], float f, ValueCodes<D, WIDE, L> &v, bool held, int t0, f16x8 (&w)[NC]) {
         const int tok = t0 + 8 * (int)((threadIdx.x & 63) >> 4);
         const bool masked = t0 + 32 > least || __any(!held);      // some column does not see all of the step
         bool nan = false;
@@ -538,7 +544,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
     }
 
     // A NaN in a token that some columns see and others do not: put into the columns that see it, taken out of the codes.
-    __device__ __forceinline__ void spread_nan(ValueCodes<D, WIDE, STREAM> &v, int tok, bool held) {
+    __device__ __forceinline__ void spread_nan(ValueCodes<D, WIDE, L> &v, int tok, bool held) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             u32x4 sees = {0u, 0u, 0u, 0u};
@@ -570,7 +576,7 @@ template <int CODE, int D, int NC, bool WIDE, bool STREAM> struct Walk {
             }
     }
 
-    __device__ __forceinline__ void accumulate(const ValueCodes<D, WIDE, STREAM> &v, const f16x8 (&w)[NC]) {   // O^T += V^T P^T
+    __device__ __forceinline__ void accumulate(const ValueCodes<D, WIDE, L> &v, const f16x8 (&w)[NC]) {   // O^T += V^T P^T
 #pragma unroll
         for (int x = 0; x < D / 64; ++x) {
             unsigned pair[4][2];                      // bytes of two tokens side by side, channel by channel

@@ -8,7 +8,7 @@
 namespace fla {
 namespace {
 
-template <int CODE, int D, int NC, int W, bool WIDE, bool STREAM>
+template <int CODE, int D, int NC, int W, bool WIDE, Loads L>
 __global__ void __launch_bounds__(W * 64, NC == 2 && D == 128 ? 3 : 2) paged_decode_kernel(const AttnParams p) {
     constexpr int kRows = 16 * NC;
     __shared__ float lds_ml[W][kRows][2];
@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(W * 64, NC == 2 && D == 128 ? 3 : 2) paged_dec
     PageWindow<WIDE> pages;
     pages.fill(p, row, t0, 32 * W);
     const Request rq = request_of(p, it.r);
-    Walk<CODE, D, NC, WIDE, STREAM> walk;
+    Walk<CODE, D, NC, WIDE, L> walk;
     walk.start(p, rq, row, head, it.tile * kRows, lds_q);
     const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
     walk.run(p, row, pages, head, t0, 32 * W, end);
@@ -162,19 +162,19 @@ __global__ void __launch_bounds__(64 * (WAVES > 4 ? WAVES : 4)) paged_join_kerne
     }
 }
 
-template <int CODE, int D, int NC, int W, bool WIDE, bool STREAM> int launch(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
+template <int CODE, int D, int NC, int W, bool WIDE, Loads L> int launch(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
     const dim3 grid((unsigned)(plan.items * p.heads));
-    FLA_LAUNCH("paged_kv_attention", stream, (paged_decode_kernel<CODE, D, NC, W, WIDE, STREAM>), grid, dim3(W * 64), 0, stream, p);
+    FLA_LAUNCH("paged_kv_attention", stream, (paged_decode_kernel<CODE, D, NC, W, WIDE, L>), grid, dim3(W * 64), 0, stream, p);
     FLA_HIP_CHECK(hipGetLastError());
     return FLA_OK;
 }
 
 template <int CODE, int D, bool WIDE> int launch_rows(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
     if (plan.nc == 1) {
-        if (plan.waves == 8) return launch<CODE, D, 1, 8, WIDE, false>(p, plan, stream);
-        return launch<CODE, D, 1, 4, WIDE, true>(p, plan, stream);
+        if (plan.waves == 8) return launch<CODE, D, 1, 8, WIDE, kAhead>(p, plan, stream);
+        return launch<CODE, D, 1, 4, WIDE, kAheadOnce>(p, plan, stream);
     }
-    return launch<CODE, D, 2, 4, WIDE, true>(p, plan, stream);
+    return launch<CODE, D, 2, 4, WIDE, kAheadOnce>(p, plan, stream);
 }
 
 template <int CODE, int D> int launch_page(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {

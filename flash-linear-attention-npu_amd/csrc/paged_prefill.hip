@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(64, 2) paged_prefill_kernel(const AttnParams p
     PageWindow<WIDE> pages;
     pages.fill(p, row, t0, 32);
     const Request rq = request_of(p, it.r);
-    Walk<CODE, D, NC, WIDE, false> walk;
+    Walk<CODE, D, NC, WIDE, kLate> walk;
     walk.start(p, rq, row, head, it.tile * kRows, lds_q);
     const int end = it.chunks == 1 ? walk.most : (int)min((int64_t)walk.most, from + (int64_t)it.units * kUnit);
     walk.run(p, row, pages, head, t0, 32, end);
