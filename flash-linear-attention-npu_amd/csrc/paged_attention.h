@@ -30,6 +30,7 @@ struct AttnParams {
     // at least min_units.  target 0: one chunk for each tile.
     int target, few, min_units;
     int tiles_each;                // tiles of a request without cu
+    int items;                     // that the grid and the workspace have room for
     float scale2;                  // scale * log2(e)
     bool clear_tail;
 };
@@ -652,14 +653,18 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
     }
 };
 
-// Rows behind the last request: 0, lse -inf.  Workgroup `part` of `parts` takes every parts-th row.
+// Rows behind the last request (and before the first, should cu not begin at 0): 0, lse -inf.  Workgroup `part` of `parts`
+// takes every parts-th row.
 template <int THREADS> __device__ __forceinline__ void clear_tail(const AttnParams &p, int head, int D, int part, int parts) {
-    for (int64_t t = (int64_t)min(max(p.cu[p.n], 0), p.tokens) + part; t < p.tokens; t += parts)
+    const int64_t first = min(max(p.cu[0], 0), p.tokens), last = min(max(p.cu[p.n], (int)first), p.tokens);
+    for (int64_t row = part; row < first + p.tokens - last; row += parts) {
+        const int64_t t = row < first ? row : row - first + last;
         for (int x = threadIdx.x; x < p.group * D; x += THREADS) {
             const int h = head * p.group + x / D, d = x % D;
             static_cast<elem *>(p.out)[t * p.o_t + h * p.o_h + d] = (elem)0.f;
             if (p.lse && d == 0) p.lse[t * p.lse_t + h * p.lse_h] = kNegInf;
         }
+    }
 }
 
 struct AttnLaunch {

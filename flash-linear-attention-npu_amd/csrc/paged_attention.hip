@@ -82,7 +82,7 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
     }
     plan.items = plan.tiles + p.target;
     FLA_REQUIRE(capacity <= INT32_MAX - 65536, FLA_ERR_SHAPE, "%s: a row of block_table names more than 2^31 - 2^16 tokens.", op);
-    FLA_REQUIRE(plan.items * shape.heads < ((int64_t)1 << 31), FLA_ERR_SHAPE, "%s: too many query rows.", op);
+    FLA_REQUIRE(plan.items * shape.heads * 64 * (prefill ? 1 : plan.waves) < ((int64_t)1 << 32), FLA_ERR_SHAPE, "%s: too many query rows.", op);
     plan.o_bytes = p.target ? (uint64_t)plan.items * shape.heads * rows * dim * 4 : 0;
     plan.bytes = p.target ? plan.o_bytes + (uint64_t)plan.items * shape.heads * rows * 8 : 0;
     if (query) {
@@ -129,6 +129,7 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
     p.heads = (int)shape.heads;
     p.pool = (uint32_t)shape.pool;
     p.scale2 = (float)(scale * 1.44269504088896340736);
+    p.items = (int)plan.items;
     p.clear_tail = clear_tail && p.cu;
     const bool f16_rows = q->dtype == FLA_F16;
     if (prefill) rc = f16_rows ? launch_paged_prefill_f16(p, plan, stream) : launch_paged_prefill(p, plan, stream);

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(64 * (WAVES > 4 ? WAVES : 4)) paged_join_kerne
     int base;
     const int head = blockIdx.x % p.heads;
     const Item it = find_item<ROWS>(p, blockIdx.x / p.heads, true, base);
-    if (!it.found || it.chunks == 1) return;
+    if (!it.found || it.chunks == 1 || base < 0 || base > p.items - it.chunks) return;    // the last two: cu_seqlens that descend
     const Request rq = request_of(p, it.r);
     const float unit = scale_unit(p, p.table + it.r * p.table_s, head);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rows = min(ROWS, rq.rows - it.tile * ROWS);

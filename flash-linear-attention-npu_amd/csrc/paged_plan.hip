@@ -180,8 +180,8 @@ int plan_impl(const fla_tensor *context, const fla_tensor *query, const fla_tens
     if ((rc = vec(op, cu, "cu_seqlens", FLA_I32, n + 1))) return rc;
     if ((rc = vec(op, seq, "seq_lens", FLA_I32, n))) return rc;
     if ((rc = vec(op, used, "blocks_used", FLA_I32, 1))) return rc;
-    FLA_REQUIRE(present(state_rows) == present(state_indices), FLA_ERR_NULL, "%s: state_rows and state_indices go together.", op);
-    if (present(state_rows)) {
+    FLA_REQUIRE(tokens == 0 || present(state_rows) == present(state_indices), FLA_ERR_NULL, "%s: state_rows and state_indices go together.", op);
+    if (tokens && present(state_rows)) {
         if ((rc = vec(op, state_rows, "state_rows", FLA_I32, n))) return rc;
         if ((rc = vec(op, state_indices, "state_indices", FLA_I32, tokens))) return rc;
     }

@@ -208,7 +208,7 @@ int rotary_impl(const fla_tensor *q, const fla_tensor *k, const fla_tensor *posi
     p.pairs = (int)pairs;
     p.tokens_per_wg = tokens >= 4096 ? kMaxTokens : 1;
     const int64_t groups = (tokens + p.tokens_per_wg - 1) / p.tokens_per_wg;
-    FLA_REQUIRE(groups < ((int64_t)1 << 31), FLA_ERR_SHAPE, "%s: too many tokens.", op);
+    FLA_REQUIRE(groups * kThreads < ((int64_t)1 << 32), FLA_ERR_SHAPE, "%s: too many tokens.", op);
     const dim3 grid((unsigned)groups);
     if (q->dtype == FLA_BF16) launch<bf16>(p, piece, grid, stream);
     else if (q->dtype == FLA_F16) launch<f16>(p, piece, grid, stream);

@@ -220,6 +220,7 @@ def rotary_axes(q, k, positions, inv_freq, sections, *, axis_order="blocked", pa
     axes in turn while they have any left (``"interleaved"``).  Channel pair j turns by ``positions[axis_j] * inv_freq[j]``
     (formed in 64 bits); a pair is channels j and j + R/2 (``pairing="half"``) or 2j and 2j + 1 (``"adjacent"``).  Channels
     from R on pass through.  Returns the rotated q and k in the memory order of the inputs."""
+    _paged_kv._refuse_grad("rotary_axes", inv_freq=inv_freq)
     if _has_tensor_requiring_grad(q, k):
         return _rotary_function().apply(q, k, positions, inv_freq, sections, axis_order, pairing)
     return _paged_kv._rotate(q, k, positions, inv_freq, sections, axis_order, pairing, False)

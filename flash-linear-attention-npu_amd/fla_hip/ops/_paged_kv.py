@@ -223,7 +223,7 @@ def paged_kv_attention(query, key_cache, value_cache, key_scales, value_scales, 
     request's q rows is token ``seq_lens - q + j`` and sees the tokens up to itself; pages that the table gives a number
     outside the pool are not seen, and a row that sees nothing is 0 with lse -inf.  ``scale`` defaults to ``D ** -0.5``.
     ``max_query_len``: the largest number of query rows of a request, if the caller knows it; it only chooses the kernel.
-    Rows behind the last request are 0 in a new result and left as they are in a given ``out``.  Returns ``out`` or, with
+    Rows that belong to no request are 0 in a new result and left as they are in a given ``out``.  Returns ``out`` or, with
     ``return_lse``, ``(out, lse)`` with lse fp32 ``[T, Hq]`` (natural logarithm)."""
     import torch
 

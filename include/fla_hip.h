@@ -819,7 +819,7 @@ int fla_rotary_axes(
  * A page's scale is the smallest power of two s (at least 2^-126) with max|x| / s <= 448 (e4m3) or 127 (int8) over the
  * finite elements stored so far in that page and head, 0 while all are 0; when it grows, the codes already there are
  * converted to it.  Codes are x / s rounded to nearest even; infinities store the largest code, NaN stores NaN (e4m3)
- * or 0 (int8). */
+ * or 0 (int8).  Rows of the caches and elements of the scales must not overlap; T < 2^26. */
 int fla_paged_kv_append(
     const fla_tensor *key, const fla_tensor *value, const fla_tensor *key_cache, const fla_tensor *value_cache,
     const fla_tensor *key_scales, const fla_tensor *value_scales, const fla_tensor *slot_mapping, void *stream);
@@ -830,8 +830,8 @@ int fla_paged_kv_append(
  * of the q rows of request r is token seq_lens[r] - q + j and sees the tokens up to itself.  Pages that block_table
  * ([N,M] i32) gives a number outside the pool are not seen.  A row that sees nothing is 0 with lse -inf.  lse f32 [T,Hq]
  * optional: natural logarithm of the sum of exponentials.  max_query_len: the largest number of query rows of a request
- * (a hint that chooses the kernel; 0: unknown).  Rows behind the last request are left as they are, or set to 0 (lse
- * -inf) with clear_tail.  Codes behind a request's last token are never read into a result. */
+ * (a hint that chooses the kernel; 0: unknown).  Rows that belong to no request (before cu_seqlens[0] or from
+ * cu_seqlens[N] on) are left as they are, or set to 0 (lse -inf) with clear_tail.  Codes behind a request's last token are never read into a result. */
 int fla_paged_kv_attention_get_workspace_size(
     const fla_tensor *query, const fla_tensor *key_cache, const fla_tensor *value_cache,
     const fla_tensor *key_scales, const fla_tensor *value_scales, const fla_tensor *block_table,

@@ -317,3 +317,40 @@ def test_oracle_plan_closed_form():
     got = ref.plan([16, 3], [2, 15], table, [9, 8], 16, 18, [5, 6])
     assert got["slots"].tolist() == [9 * 16, 9 * 16 + 1] + list(range(7 * 16 + 3, 7 * 16 + 16)) + [8 * 16, 8 * 16 + 1, -1]
     assert got["table"].tolist() == [[4, 9], [7, 8]] and got["used"].tolist() == [2] and got["states"].tolist() == [5, 5] + [6] * 15 + [-1]
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(kc=desc((10, 2, 16, 128), I8, (4096, 0, 128, 1))), "rows of key_cache overlap"),
+    (dict(vc=desc((10, 2, 16, 128), I8, (0, 2048, 128, 1))), "rows of value_cache overlap"),
+    (dict(vs=desc((10, 2), F32, (0, 1))), "elements of value_scales overlap"),
+    (dict(key=desc((1 << 26, 2, 128), BF16), value=desc((1 << 26, 2, 128), BF16), slots=desc((1 << 26,), I64)), "too many tokens"),
+])
+def test_append_refuses_caches_that_overlap_and_too_many_tokens(lib, change, text):
+    from fla_hip.ops import _paged_kv as P
+
+    fn = lib.fla_paged_kv_append
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["paged_kv_append"], ctypes.c_void_p], ctypes.c_int
+    assert fn(*append_args(**change), None) == SHAPE and text in lib.fla_last_error().decode()
+
+
+def test_grids_beyond_the_launch_limit_are_refused(lib):
+    n = 1 << 23                                         # times two heads of 256 threads: 2^32
+    big = dict(query=desc((n, 8, 128), BF16), out=desc((n, 8, 128), BF16), lse=None, block_table=desc((n, 4), I32), seq_lens=desc((n,), I32),
+               cu_seqlens=None)
+    status, _, text = query(lib, attention_args(**big))
+    assert status == SHAPE and "too many query rows" in text
+    from fla_hip.ops import _paged_kv as P
+
+    tokens = 1 << 26                                    # four to a workgroup of 256 threads: 2^32
+    args, keep = rotary_args(q=desc((tokens, 2, 16), BF16), q_out=desc((tokens, 2, 16), BF16), k=None, k_out=None, positions=desc((2, tokens), I64))
+    fn = lib.fla_rotary_axes
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["rotary_axes"], ctypes.c_void_p], ctypes.c_int
+    assert fn(*args, None) == SHAPE and "too many tokens" in lib.fla_last_error().decode()
+
+
+def test_rotary_refuses_frequencies_that_want_a_gradient():
+    from fla_hip import ops
+
+    q, freq = torch.zeros(5, 2, 16, dtype=torch.bfloat16), torch.ones(4, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="no gradient is bound for inv_freq"):
+        ops.rotary_axes(q, None, torch.zeros(1, 5, dtype=torch.int64), freq, (4,))

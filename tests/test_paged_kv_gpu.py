@@ -788,3 +788,35 @@ def test_refusals_of_gradients_and_cpu_tensors(dev):
         ops.paged_kv_attention(q, kc, kc, ks, ks, table, lens, out=torch.empty(1, 2, 64, device=dev, dtype=BF))
     with pytest.raises(TypeError, match="key_cache must be a ROCm GPU tensor"):
         ops.paged_kv_attention(q.detach(), kc.cpu(), kc, ks, ks, table, lens)
+
+
+def test_plan_without_tokens_keeps_its_state_rows_apart(dev):
+    from fla_hip import ops
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    table = torch.full((2, 2), -1, dtype=torch.int32, device=dev)
+    slots, pos, cu, seq, used, states = ops.paged_kv_plan(i32([4, 0]), i32([0, 3]), table, i32([7]), 16, 0, state_rows=i32([1, 0]))
+    assert slots.numel() == pos.numel() == states.numel() == 0 and states.dtype == torch.int32
+    assert cu.tolist() == [0, 0, 3] and seq.tolist() == [4, 3] and used.tolist() == [1] and table.tolist() == [[-1, -1], [7, -1]]
+
+
+@pytest.mark.parametrize("new", [2, 40])
+def test_rows_before_the_first_request(dev, new):
+    from fla_hip import ops
+    rng, gen = random.Random(3), torch.Generator().manual_seed(3)
+    page, heads, kv_heads, dim, lens = 16, 4, 2, 64, [50, 43]
+    cu = [3, 3 + new, 3 + 2 * new]
+    kc, ks = random_cache(gen, 9, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, 9, kv_heads, page, dim, E4M3, dev)
+    table = make_table(rng, lens, page, 4, 9)
+    q = torch.randn(cu[-1] + 2, heads, dim, generator=gen).to(BF)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    args = (q.to(dev), kc, vc, ks, vs, table.to(dev), i32(lens), i32(cu))
+    torch.empty(1 << 20, dtype=BF, device=dev).fill_(7.0)             # what a new result may find in its memory
+    out, lse = ops.paged_kv_attention(*args, max_query_len=new, return_lse=True)
+    for rows in (slice(0, 3), slice(cu[-1], None)):
+        assert bool((out[rows] == 0).all()) and bool((lse[rows] == -math.inf).all())
+    mine = slice(3, cu[-1])
+    check_attention(dev, q[mine], (kc, vc, ks, vs), table, lens, [c - 3 for c in cu], dim ** -0.5, got=(out[mine], lse[mine]))
+    given = torch.full_like(q, 3.0).to(dev)
+    ops.paged_kv_attention(*args, out=given, max_query_len=new)
+    assert torch.equal(given[mine], out[mine]) and bool((given[:3] == 3).all()) and bool((given[cu[-1]:] == 3).all())
