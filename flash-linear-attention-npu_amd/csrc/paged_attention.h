@@ -383,12 +383,18 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
             Place<WIDE> at = pages.get(p, row, t0, stride, 0, most);
             k.load(p, head, t0, at, off);
             // Steps that every column sees whole, and that move no maximum, have a loop of their own: with the code for the
-            // others in it, the compiler keeps the accumulators in memory for part of it.
+            // others in it, the compiler keeps the accumulators in memory for part of it.  The products go before the other
+            // wave's vector instructions (s_setprio): the matrix unit is asked first while there is something for it, and the
+            // two waves of a SIMD fall out of step (prefill of 2 x 4096 tokens, 32 heads on 8: D = 128 849 us without, 770 us with
+            // it, int8 970 and 870; D = 64 571 and 533; but D = 256, whose products are longer, 1970 and 2063).
+            constexpr bool kProductsFirst = D <= 128;
             for (int step = 1; t0 < end;) {
                 while (t0 < end && t0 + 32 <= least && !fresh) {
                     v.load(p, head, t0, at, off);
                     f32x4 s[NC][2];
+                    if (kProductsFirst) __builtin_amdgcn_s_setprio(1);
                     scores(k, s);
+                    if (kProductsFirst) __builtin_amdgcn_s_setprio(0);
                     const float f = k.scale * p.scale2, floor = unit * 0x1p-60f;
                     const float add = __builtin_amdgcn_logf(v.scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(v.scale);
                     f16x8 w[NC];
@@ -402,7 +408,9 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
 #pragma unroll
                     for (int c = 0; c < NC; ++c) l[c] = fmaf(sum[c], back, l[c]);
                     advance(p, row, pages, head, t0, stride, end, step, at, k, off);
+                    if (kProductsFirst) __builtin_amdgcn_s_setprio(1);
                     accumulate(v, w);
+                    if (kProductsFirst) __builtin_amdgcn_s_setprio(0);
                 }
                 if (t0 >= end) break;
                 v.load(p, head, t0, at, off);
