@@ -68,8 +68,8 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
     //    least 1024 tokens, where tiles alone fill the chip, since ragged requests balance better (32 heads on 8 of 128,
     //    e4m3: one request of 262 k tokens 102 us with 512 and 115 us with 2048 workgroups; 128 requests of up to 8 k 239
     //    and 211 us);
-    //  - tables of at most 2048 tokens: one chunk and one launch, of eight waves (four requests of 1100: 11.8 us against 12 us
-    //    with two launches on the GPU, and one launch less on the host);
+    //  - tables of at most 2048 tokens: one chunk and one launch, of eight waves (four requests of 1100: 11.6 us against 10.2
+    //    to 12.3 us with two launches on the GPU, and one launch less on the host);
     //  - prefill: only where tiles, of one wave each, would leave compute units idle.
     const int64_t capacity = table->shape[1] << shape.shift, tiles_all = plan.tiles * shape.heads;
     plan.waves = 4;

@@ -5,7 +5,8 @@
 // lengths for itself (two prefix sums over tiles of 1024 requests in LDS) instead of waiting for another one's sums, then
 // fills the pieces of 256 tokens and of 256 new pages that fall to it; a token finds its request by
 // bisection in the tile's sums.  A slot in a page that this step opens is computed from the free list, never read back
-// from the table, so no workgroup depends on another's writes.
+// from the table, so no workgroup depends on another's writes.  Measured: 256 requests of one token 5.6 us, 64 requests of 110 k
+// tokens in pages of 16 6.4 us (a launch alone: 1.8 us); four tokens a thread: 9.7 us.
 #include "common.h"
 #include "device_utils.h"
 

@@ -1,7 +1,10 @@
 // paged_kv_attention for many query rows (chunked prefill): a wave takes 64 of them (32 for D = 256) over all their keys.
 // Bound by the vector and matrix units together.  For a 32-token step and D = 128 a wave issues 64 matrix instructions
-// (1024 clocks of the matrix pipe) and about 350 vector ones; codes are widened once for 64 rows, straight from the loads
-// of the wave, with no LDS and no barrier: the tiles of a head run on one XCD, whose L2 holds its keys.
+// (1024 clocks of the matrix pipe) and about 230 vector ones, 32 of them exponentials; codes are widened once for 64 rows,
+// straight from the loads of the wave, with no LDS (but for the queries, which would take registers) and no barrier: the
+// tiles of a head run on one XCD, whose L2 holds its keys.  32 rows a wave: 1150 us where 64 take 852.
+// Measured: 2 x 4096 tokens behind 4096, 32 heads on 8 of 128, e4m3: 766 us = 1077 TFLOP/s, 77 % of what a library product of
+// 8192^3 reaches; int8 870 us; D = 64 533 us; D = 256 1950 us.
 #include "paged_attention.h"
 
 namespace fla {

@@ -2,7 +2,8 @@
 //   angle(t, j) = positions[axis(j), t] * inv_freq[j];   (a, b) -> (a cos - b sin, b cos + a sin);   gradient: -angle
 // Every element is read once and written once: bound by HBM.  A workgroup takes a few tokens: it forms their R/2 sines and
 // cosines once in LDS (the angle in 64 bits, reduced to a fraction of a turn before the fp32 sine, since positions run to
-// millions), then streams the rows of all heads of q and k past them, 16 bytes per load.
+// millions), then streams the rows of all heads of q and k past them, 16 bytes per load.  Measured: 32768 tokens, 32 + 8 heads of
+// 128, half of the channels turned, bf16: 130 us for 670 MB = 5.2 TB/s, the rate of a copy; 256 tokens: 4.8 us.
 #include "common.h"
 #include "device_utils.h"
 
