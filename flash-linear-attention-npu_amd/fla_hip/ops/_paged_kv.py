@@ -126,7 +126,8 @@ def paged_kv_plan(context_lens, query_lens, block_table, free_blocks, block_size
     slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
     # the int32 results are parts of one allocation
     sizes = [num_tokens, n + 1, n, 1] if state_rows is None else [num_tokens, n + 1, n, 1, num_tokens]
-    positions, cu, seq, used, *rest = torch.empty(sum(sizes), dtype=i32, device=dev).split_with_sizes(sizes)
+    ints = torch.empty(sum(sizes), dtype=i32, device=dev)
+    positions, cu, seq, used, *rest = ints.split_with_sizes(sizes)
     states = rest[0] if rest else None
     if n == 0:
         slots.fill_(-1)
@@ -135,10 +136,12 @@ def paged_kv_plan(context_lens, query_lens, block_table, free_blocks, block_size
         if states is not None:
             states.fill_(-1)
         return slots, positions, cu, seq, used, states
-    d = call.tensor
+    d, at = call.tensor, ints.data_ptr()
+    new = lambda first, count: _FLA_TENSOR[1].pack(at + 4 * first, _CODES["torch.int32"], 1, count, 1)
     call.run("paged_kv_plan", d(context_lens, "context_lens"), d(query_lens, "query_lens"), d(block_table, "block_table"),
-             d(free_blocks, "free_blocks"), d(state_rows, "state_rows"), block_size, d(slots, "slot_mapping"), d(positions, "positions"),
-             d(cu, "cu_seqlens"), d(seq, "seq_lens"), d(used, "blocks_used"), d(states, "state_indices"))
+             d(free_blocks, "free_blocks"), d(state_rows, "state_rows"), block_size, d(slots, "slot_mapping"), new(0, num_tokens),
+             new(num_tokens, n + 1), new(num_tokens + n + 1, n), new(num_tokens + 2 * n + 1, 1),
+             None if states is None else new(num_tokens + 2 * n + 2, num_tokens))
     return slots, positions, cu, seq, used, states
 
 
@@ -233,10 +236,11 @@ def paged_kv_attention(query, key_cache, value_cache, key_scales, value_scales, 
         raise ValueError(f"paged_kv_attention: query must be [T, Hq, D], got rank {query.dim()}.")
     clear = out is None
     if clear:
-        out = torch.empty(query.shape, dtype=query.dtype, device=call.device)
-    lse = torch.empty(query.shape[:2], dtype=torch.float32, device=call.device) if return_lse else None
-    if query.shape[0] == 0 or block_table.shape[0] == 0:
-        if cu_seqlens is None and query.shape[0] != block_table.shape[0]:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    rows, heads, dim = query.shape
+    lse = query.new_empty((rows, heads), dtype=torch.float32) if return_lse else None
+    if rows == 0 or block_table.shape[0] == 0:
+        if cu_seqlens is None and rows != block_table.shape[0]:
             raise ValueError("paged_kv_attention: without cu_seqlens query must have one row for each request.")
         if clear:
             out.zero_()
@@ -246,9 +250,12 @@ def paged_kv_attention(query, key_cache, value_cache, key_scales, value_scales, 
     if not clear and lse is not None and cu_seqlens is not None:
         lse.fill_(float("-inf"))      # rows behind the last request: `out` stays as it is, lse is new
     d = call.tensor
+    q = d(query, "query")
+    # descriptors of new results are written down: nothing about them has to be asked
+    to = _FLA_TENSOR[3].pack(out.data_ptr(), _CODE_OF[query.dtype], 3, rows, heads, dim, heads * dim, dim, 1) if clear else d(out, "out")
     call.run_with_workspace(
-        "paged_kv_attention", d(query, "query"), d(key_cache, "key_cache"), d(value_cache, "value_cache"), d(key_scales, "key_scales"),
+        "paged_kv_attention", q, d(key_cache, "key_cache"), d(value_cache, "value_cache"), d(key_scales, "key_scales"),
         d(value_scales, "value_scales"), d(block_table, "block_table"), d(seq_lens, "seq_lens"), d(cu_seqlens, "cu_seqlens"),
-        query.shape[-1] ** -0.5 if scale is None else float(scale), 0 if max_query_len is None else int(max_query_len), clear,
-        d(out, "out"), d(lse, "lse"))
+        dim ** -0.5 if scale is None else float(scale), 0 if max_query_len is None else int(max_query_len), clear, to,
+        None if lse is None else _FLA_TENSOR[2].pack(lse.data_ptr(), _CODES["torch.float32"], 2, rows, heads, heads, 1))
     return (out, lse) if return_lse else out
