@@ -248,8 +248,8 @@ template <int D, bool WIDE, Loads L> struct ValueCodes {
     __device__ __forceinline__ void load(const AttnParams &p, int head, int t0, const Place<WIDE> &pl, const LaneOffsets &off) {
         typedef unsigned VV __attribute__((ext_vector_type(D / 64)));
         const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, in_page = (1 << p.shift) - 1;
-        const float s = p.vs[(int64_t)pl.page * p.vs_p + head * p.vs_h];
-        scale = pl.held ? s : 0.f;
+        scale = p.vs[(int64_t)pl.page * p.vs_p + head * p.vs_h];      // raw: any use here would wait for all loads in flight
+        // (prefill of 2 x 4096: 760 us with a select here, 745 us without; D = 256 1958 and 1800)
         const uint8_t *at = p.vc + (int64_t)pl.page * p.vc_p + (int64_t)head * p.vc_h;
         if (WIDE) at += (int64_t)(t0 & in_page) * p.vc_t;
         else at += (int64_t)((t0 + 8 * g) & in_page) * p.vc_t + i * (D / 16);
@@ -362,13 +362,13 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
                 const int t1 = t0 + stride;
                 const bool go = t1 < end;
                 f32x4 s[NC][2];
-                Place<WIDE> next = at;
                 scores(k, s);
                 const float f = k.scale * p.scale2;
-                if (go) {
-                    next = pages.get(p, row, t1, stride, step, most);
-                    k.load(p, head, t1, next, off);
-                }
+                // Never behind a branch, or the values of this step would wait for these loads too (48 requests of 1 to 7 rows
+                // 31.0 us, 29.6 us so; one row each 25.2 and 23.6); after the last step all lanes load one piece seen already.
+                const Place<WIDE> next = pages.get(p, row, t1, stride, step, most);
+                const LaneOffsets there = {go ? off.k : 0u, off.v};
+                k.load(p, head, go ? t1 : t0, go ? next : at, there);
                 f16x8 w[NC];
                 weigh(s, f, v, at.held, t0, w);
                 accumulate(v, w);
@@ -386,15 +386,14 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
             // others in it, the compiler keeps the accumulators in memory for part of it.  The products go before the other
             // wave's vector instructions (s_setprio): the matrix unit is asked first while there is something for it, and the
             // two waves of a SIMD fall out of step (prefill of 2 x 4096 tokens, 32 heads on 8: D = 128 849 us without, 770 us with
-            // it, int8 970 and 870; D = 64 571 and 533; but D = 256, whose products are longer, 1970 and 2063).
-            constexpr bool kProductsFirst = D <= 128;
+            // it, int8 970 and 870; D = 64 571 and 533; D = 256 1815 and 1793).
             for (int step = 1; t0 < end;) {
                 while (t0 < end && t0 + 32 <= least && !fresh) {
                     v.load(p, head, t0, at, off);
                     f32x4 s[NC][2];
-                    if (kProductsFirst) __builtin_amdgcn_s_setprio(1);
+                    __builtin_amdgcn_s_setprio(1);
                     scores(k, s);
-                    if (kProductsFirst) __builtin_amdgcn_s_setprio(0);
+                    __builtin_amdgcn_s_setprio(0);
                     const float f = k.scale * p.scale2, floor = unit * 0x1p-60f;
                     const float add = __builtin_amdgcn_logf(v.scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(v.scale);
                     f16x8 w[NC];
@@ -408,9 +407,9 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
 #pragma unroll
                     for (int c = 0; c < NC; ++c) l[c] = fmaf(sum[c], back, l[c]);
                     advance(p, row, pages, head, t0, stride, end, step, at, k, off);
-                    if (kProductsFirst) __builtin_amdgcn_s_setprio(1);
+                    __builtin_amdgcn_s_setprio(1);
                     accumulate(v, w);
-                    if (kProductsFirst) __builtin_amdgcn_s_setprio(0);
+                    __builtin_amdgcn_s_setprio(0);
                 }
                 if (t0 >= end) break;
                 v.load(p, head, t0, at, off);
@@ -521,8 +520,8 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
         float by[NC];                      // what sums and accumulators are multiplied by
 #pragma unroll
         for (int c = 0; c < NC; ++c) by[c] = 1.f;
-        const float floor = unit * 0x1p-60f, scale = fmaxf(v.scale, floor), add = __builtin_amdgcn_logf(scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(scale);
-        const bool tiny = __any(!(v.scale >= floor)), early = masked || fresh;
+        const float floor = unit * 0x1p-60f, page_scale = held ? v.scale : 0.f, scale = fmaxf(page_scale, floor), add = __builtin_amdgcn_logf(scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(scale);
+        const bool tiny = __any(!(page_scale >= floor)), early = masked || fresh;
         bool moved = early;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -534,7 +533,7 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
                 moved = true;
                 w[c] = exponentials(s[c], f, add - m[c], sum);
             }
-            if (__builtin_expect(tiny, 0)) w[c] = exponentials(s[c], f, add - m[c], sum, v.scale >= floor ? 1.f : v.scale / floor);
+            if (__builtin_expect(tiny, 0)) w[c] = exponentials(s[c], f, add - m[c], sum, page_scale >= floor ? 1.f : page_scale / floor);
             l[c] = fmaf(sum, back, l[c] * by[c]);
         }
         if (__builtin_expect(fresh, 0)) {

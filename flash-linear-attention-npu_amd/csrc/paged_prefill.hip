@@ -3,8 +3,8 @@
 // (1024 clocks of the matrix pipe) and about 230 vector ones, 32 of them exponentials; codes are widened once for 64 rows,
 // straight from the loads of the wave, with no LDS (but for the queries, which would take registers) and no barrier: the
 // tiles of a head run on one XCD, whose L2 holds its keys.  32 rows a wave: 1150 us where 64 take 852.
-// Measured: 2 x 4096 tokens behind 4096, 32 heads on 8 of 128, e4m3: 766 us = 1077 TFLOP/s, 77 % of what a library product of
-// 8192^3 reaches; int8 870 us; D = 64 533 us; D = 256 1950 us.
+// Measured: 2 x 4096 tokens behind 4096, 32 heads on 8 of 128, e4m3: 745 to 770 us = 1070 to 1107 TFLOP/s, 76 to 79 % of what a library
+// product of 8192^3 reaches; int8 845 us; D = 64 515 us; D = 256 1793 us.
 #include "paged_attention.h"
 
 namespace fla {
