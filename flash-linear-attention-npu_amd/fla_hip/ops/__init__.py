@@ -192,21 +192,24 @@ def _rotary_function():
     import torch
 
     class RotaryAxes(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, q, k, positions, inv_freq, sections, axis_order, pairing):
-            ctx.save_for_backward(positions, inv_freq)
-            ctx.how = sections, axis_order, pairing
-            ctx.set_materialize_grads(False)
-            return _paged_kv._rotate(q, k, positions, inv_freq, sections, axis_order, pairing, False)
+        """Linear in q and k: the gradient is the inverse turn, which is an operator of the same kind."""
 
         @staticmethod
-        @torch.autograd.function.once_differentiable
+        def forward(ctx, q, k, positions, inv_freq, sections, axis_order, pairing, inverse):
+            ctx.save_for_backward(positions, inv_freq)
+            ctx.how = sections, axis_order, pairing, not inverse
+            ctx.set_materialize_grads(False)
+            return _paged_kv._rotate(q, k, positions, inv_freq, sections, axis_order, pairing, inverse)
+
+        @staticmethod
         def backward(ctx, dq, dk):
-            grads = [g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk)]
-            if grads[0] is None:
-                grads = [None if grads[1] is None else _paged_kv._rotate(grads[1], None, *ctx.saved_tensors, *ctx.how, True)[0]]
-                return None, *grads, *[None] * 5
-            return *_paged_kv._rotate(*grads, *ctx.saved_tensors, *ctx.how, True), *[None] * 5
+            turn = RotaryAxes.apply if torch.is_grad_enabled() else _paged_kv._rotate      # enabled: a graph of the gradient is wanted
+            dq, dk = [g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk)]
+            if dq is not None:
+                dq, dk = turn(dq, dk, *ctx.saved_tensors, *ctx.how)
+            elif dk is not None:
+                dk = turn(dk, None, *ctx.saved_tensors, *ctx.how)[0]
+            return dq, dk, None, None, None, None, None, None
 
     return RotaryAxes
 
@@ -222,7 +225,7 @@ def rotary_axes(q, k, positions, inv_freq, sections, *, axis_order="blocked", pa
     from R on pass through.  Returns the rotated q and k in the memory order of the inputs."""
     _paged_kv._refuse_grad("rotary_axes", inv_freq=inv_freq)
     if _has_tensor_requiring_grad(q, k):
-        return _rotary_function().apply(q, k, positions, inv_freq, sections, axis_order, pairing)
+        return _rotary_function().apply(q, k, positions, inv_freq, sections, axis_order, pairing, False)
     return _paged_kv._rotate(q, k, positions, inv_freq, sections, axis_order, pairing, False)
 
 

@@ -820,3 +820,24 @@ def test_rows_before_the_first_request(dev, new):
     given = torch.full_like(q, 3.0).to(dev)
     ops.paged_kv_attention(*args, out=given, max_query_len=new)
     assert torch.equal(given[mine], out[mine]) and bool((given[:3] == 3).all()) and bool((given[cu[-1]:] == 3).all())
+
+
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_rotary_gradient_has_a_gradient(dev, adjacent):
+    """The operator is linear, so the gradient of <u, dq(w)> in w is the operator itself applied to u: the same kernel on the
+    same numbers, equal to the bit."""
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(8)
+    q, w, u = (torch.randn(9, 3, 16, generator=gen).to(dev) for _ in range(3))
+    k, wk, uk = (torch.randn(9, 1, 16, generator=gen).to(dev) for _ in range(3))
+    pos, freq = torch.arange(9, device=dev)[None], torch.rand(6, generator=gen).to(dev)
+    how = dict(pairing="adjacent" if adjacent else "half")
+    q.requires_grad_(), k.requires_grad_(), w.requires_grad_(), wk.requires_grad_()
+    grads = torch.autograd.grad(ops.rotary_axes(q, k, pos, freq, (6,), **how), (q, k), (w, wk), create_graph=True)
+    again = torch.autograd.grad(grads, (w, wk), (u, uk))
+    with torch.no_grad():
+        want = ops.rotary_axes(u, uk, pos, freq, (6,), **how)
+        back = ops.rotary_axes_bwd(w, wk, pos, freq, (6,), **how)
+    assert all(torch.equal(a, b) for a, b in zip(grads, back)) and all(torch.equal(a, b) for a, b in zip(again, want))
+    only = torch.autograd.grad(ops.rotary_axes(q, k, pos, freq, (6,), **how)[1], k, wk, create_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(only, wk, uk)[0], want[1])
