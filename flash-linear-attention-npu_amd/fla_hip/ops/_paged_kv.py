@@ -37,7 +37,8 @@ class _Call:
     the call): a tenth of the time that ctypes structures take, which a decode step would otherwise spend on the host."""
 
     def __init__(self, anchor, name: str):
-        _runtime.ensure_gpu_tensor(anchor, name)
+        if not getattr(anchor, "is_cuda", False):
+            _runtime.ensure_gpu_tensor(anchor, name)
         self.device = anchor.device
         self.index = anchor.get_device()
 
@@ -69,8 +70,11 @@ class _Call:
     def run(self, name: str, *args):
         """``fla_<name>(<operands>, stream)`` on the current stream of the call's device."""
         launch = _runtime.bind_direct(name, OP_ARGTYPES[name])
-        with _runtime.device_guard(self.device):
-            status = launch(*args, _runtime.raw_stream(self.device))
+        if _runtime.is_current(self.index):
+            status = launch(*args, _runtime.raw_stream(self.index))
+        else:
+            with _runtime.device_guard(self.index):
+                status = launch(*args, _runtime.raw_stream(self.index))
         if status:
             raise RuntimeError(f"fla_{name} failed with status={status}: {_runtime.last_error()}")
 
@@ -80,12 +84,12 @@ class _Call:
 
         query, launch = _runtime._bind(name, OP_ARGTYPES[name])
         size = ctypes.c_uint64(0)
-        with _runtime.device_guard(self.device):
+        with _runtime.device_guard(self.index):
             status = query(*args, ctypes.byref(size))
             if status:
                 raise RuntimeError(f"fla_{name}_get_workspace_size failed with status={status}: {_runtime.last_error()}")
             workspace = torch.empty(size.value, dtype=torch.uint8, device=self.device) if size.value else None
-            status = launch(*args, workspace.data_ptr() if workspace is not None else None, size.value, _runtime.raw_stream(self.device))
+            status = launch(*args, workspace.data_ptr() if workspace is not None else None, size.value, _runtime.raw_stream(self.index))
         if status:
             raise RuntimeError(f"fla_{name} failed with status={status}: {_runtime.last_error()}")
 
@@ -147,8 +151,11 @@ def paged_kv_plan(context_lens, query_lens, block_table, free_blocks, block_size
 
 @functools.lru_cache(maxsize=64)
 def _axis_table(sections: tuple, axis_order: str):
-    """Axis of each frequency as a host array: contiguous sections, or the axes in turn while they have any left."""
+    """Axis of each frequency as a host array: contiguous sections, or the axes in turn while they have any left.  None for
+    sections that make no sense."""
     left, got = list(sections), []
+    if any(n < 0 for n in left):
+        return None, None
     if axis_order == "blocked":
         got = [a for a, n in enumerate(left) for _ in range(n)]
     else:
@@ -169,24 +176,23 @@ def _rotate(q, k, positions, inv_freq, sections, axis_order: str, pairing: str, 
     if pairing not in ("half", "adjacent"):
         raise ValueError(f"rotary_axes: pairing must be 'half' or 'adjacent', got {pairing!r}.")
     call = _Call(q, "q")
-    sections = tuple(int(s) for s in sections)
-    if any(s < 0 for s in sections) or sum(sections) != inv_freq.numel():
+    sections = tuple(map(int, sections))
+    table = _axis_table(sections, axis_order)[1]
+    if table is None or table.size != inv_freq.numel():
         raise ValueError(f"rotary_axes: sections {sections} must be non-negative and sum to the {inv_freq.numel()} frequencies.")
     if positions.dim() < 1 or positions.shape[0] != len(sections):
         raise ValueError(f"rotary_axes: positions must have one row for each of the {len(sections)} sections.")
     q_out = torch.empty_like(q)
     k_out = None if k is None else torch.empty_like(k)
-    if q.numel() == 0 and k is None:
-        return q_out, k_out
     if q.numel() == 0 or (k is not None and k.numel() == 0):      # one of the two is empty: the other goes alone
         if q.numel():
             return _rotate(q, None, positions, inv_freq, sections, axis_order, pairing, inverse)[0], k_out
-        if k.numel():
+        if k is not None and k.numel():
             return q_out, _rotate(k, None, positions, inv_freq, sections, axis_order, pairing, inverse)[0]
         return q_out, k_out
     d = call.tensor
     call.run("rotary_axes", d(q, "q"), d(k, "k"), d(positions, "positions"), d(inv_freq, "inv_freq"),
-             ctypes.addressof(_axis_table(sections, axis_order)[1]), pairing == "adjacent", inverse, d(q_out, "q_out"), d(k_out, "k_out"))
+             ctypes.addressof(table), pairing == "adjacent", inverse, d(q_out, "q_out"), d(k_out, "k_out"))
     return q_out, k_out
 
 

@@ -216,18 +216,25 @@ def bind_direct(name: str, argtypes: Sequence):
 _HERE = contextlib.nullcontext()
 
 
-def device_guard(device):
-    """Makes ``device`` current for the time of a call; nothing to do where it is already."""
+def is_current(index: int) -> bool:
+    """Whether the GPU with this number, of which a tensor exists already, is the calling thread's current device."""
     import torch
 
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return torch._C._cuda_getDevice() == index
 
 
-def raw_stream(device) -> int:
-    """The ``hipStream_t`` of torch's current stream on ``device``, without making a ``torch.cuda.Stream`` for it."""
+def device_guard(index: int):
+    """Makes a device current for the time of a call; nothing to do where it is already."""
     import torch
 
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return _HERE if is_current(index) else torch.cuda.device(index)
+
+
+def raw_stream(index: int) -> int:
+    """The ``hipStream_t`` of torch's current stream on a device, without making a ``torch.cuda.Stream`` for it."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def call_op_noalloc(name: str, argtypes: Sequence, build_args: Callable[[CallContext], list], outputs):
