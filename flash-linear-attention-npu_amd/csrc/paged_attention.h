@@ -243,13 +243,17 @@ template <int D, bool WIDE, Loads L> struct KeyCodes {
 };
 
 template <int D, bool WIDE, Loads L> struct ValueCodes {
+    static constexpr bool kRaw = L == kLate || D == 64;
     unsigned c[8][D / 64];
-    float scale;
+    float scale;           // kRaw: of page 0 where nothing is held
     __device__ __forceinline__ void load(const AttnParams &p, int head, int t0, const Place<WIDE> &pl, const LaneOffsets &off) {
         typedef unsigned VV __attribute__((ext_vector_type(D / 64)));
         const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15, in_page = (1 << p.shift) - 1;
-        scale = p.vs[(int64_t)pl.page * p.vs_p + head * p.vs_h];      // raw: any use here would wait for all loads in flight
-        // (prefill of 2 x 4096: 760 us with a select here, 745 us without; D = 256 1958 and 1800)
+        // The use of the scale here makes the loads below wait for those before them.  That holds a prefill up (2 x 4096: 760 us
+        // with it, 745 us without; D = 256 1958 and 1800) and decode with D = 64, but larger heads decode faster with it (48
+        // requests of 1 to 7 rows, D = 128: 47.5 and 51 us; 256 of 2500 tokens 155 and 159 us).
+        const float s = p.vs[(int64_t)pl.page * p.vs_p + head * p.vs_h];
+        scale = kRaw || pl.held ? s : 0.f;
         const uint8_t *at = p.vc + (int64_t)pl.page * p.vc_p + (int64_t)head * p.vc_h;
         if (WIDE) at += (int64_t)(t0 & in_page) * p.vc_t;
         else at += (int64_t)((t0 + 8 * g) & in_page) * p.vc_t + i * (D / 16);
@@ -364,11 +368,16 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
                 f32x4 s[NC][2];
                 scores(k, s);
                 const float f = k.scale * p.scale2;
-                // Never behind a branch, or the values of this step would wait for these loads too (48 requests of 1 to 7 rows
-                // 31.0 us, 29.6 us so; one row each 25.2 and 23.6); after the last step all lanes load one piece seen already.
-                const Place<WIDE> next = pages.get(p, row, t1, stride, step, most);
-                const LaneOffsets there = {go ? off.k : 0u, off.v};
-                k.load(p, head, go ? t1 : t0, go ? next : at, there);
+                // D = 64: not behind a branch, or the values of this step would wait for these loads too; after the last step all
+                // lanes load one piece seen already (48 requests of 1 to 7 rows 31.0 us behind a branch, 29.6 us so; one row each
+                // 25.2 and 23.6).  For larger heads the last loads cost more than the wait (48 requests of 1 to 7 rows, D = 128:
+                // 47.4 and 49.6 us; 256 of 2500 tokens 154 and 157 us).
+                Place<WIDE> next = at;
+                if (D == 64 || go) {
+                    const Place<WIDE> behind = pages.get(p, row, t1, stride, step, most);
+                    if (go) next = behind;
+                    k.load(p, head, go ? t1 : t0, next, {go ? off.k : 0u, off.v});
+                }
                 f16x8 w[NC];
                 weigh(s, f, v, at.held, t0, w);
                 accumulate(v, w);
@@ -520,7 +529,7 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
         float by[NC];                      // what sums and accumulators are multiplied by
 #pragma unroll
         for (int c = 0; c < NC; ++c) by[c] = 1.f;
-        const float floor = unit * 0x1p-60f, page_scale = held ? v.scale : 0.f, scale = fmaxf(page_scale, floor), add = __builtin_amdgcn_logf(scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(scale);
+        const float floor = unit * 0x1p-60f, page_scale = !ValueCodes<D, WIDE, L>::kRaw || held ? v.scale : 0.f, scale = fmaxf(page_scale, floor), add = __builtin_amdgcn_logf(scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(scale);
         const bool tiny = __any(!(page_scale >= floor)), early = masked || fresh;
         bool moved = early;
 #pragma unroll
