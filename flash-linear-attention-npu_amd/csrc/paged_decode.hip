@@ -3,8 +3,9 @@
 // Bound by HBM: each code is read once, with loads that leave the caches alone (a code is not read again in this call).  The
 // waves of a workgroup take 32-token steps of a chunk in turn, each with its own running maximum, sum and accumulators (the
 // walk of paged_attention.h: no LDS, no barrier), and are joined once at the end.
-// Measured, 32 heads on 8 of 128: 128 ragged requests to 8192 tokens 187 us + 5.6 us of join for 1.04 GB; one of 262 k tokens 89 + 5.4 us for
-// 537 MB; four to 1100 tokens 12.0 us (five steps of a memory latency, 1.2 us, each); 48 requests of 1 to 7 rows 23 + 6.8 us.
+// Measured, 32 heads on 8 of 128: 128 ragged requests to 8192 tokens 187 us + 5.6 us of join for 1.04 GB; one of 262 k tokens
+// 89 + 5.4 us for 537 MB; four to 1100 tokens 12.0 us (32 workgroups, five steps of 1.2 us: the vector instructions of
+// eight waves); 24 heads on 4 of 64, 48 requests of 1 to 7 rows 23 + 6.6 us.
 #include "paged_attention.h"
 
 namespace fla {
