@@ -37,7 +37,7 @@ struct AttnParams {
 
 struct Request {
     int first, rows, units;        // first query token, query rows (tokens * group), key units
-    int len, new_tokens;           // cached tokens that the table can name, query tokens
+    int len, new_tokens;           // cached tokens, query tokens from `first` on: also those behind the last row of q
 };
 
 __device__ __forceinline__ Request request_of(const AttnParams &p, int r) {
@@ -48,7 +48,8 @@ __device__ __forceinline__ Request request_of(const AttnParams &p, int r) {
         b = min(max(p.cu[r + 1], a), p.tokens);
     }
     q.first = a;
-    q.new_tokens = b - a;
+    // Row j of a request is token len - (query tokens) + j also where q ends inside the request: the rows that q lacks count.
+    q.new_tokens = p.cu ? max(p.cu[r + 1], a) - a : 1;
     q.rows = (b - a) * p.group;
     const int64_t most = (int64_t)p.width << p.shift;
     q.len = max(p.lens[r], 0);

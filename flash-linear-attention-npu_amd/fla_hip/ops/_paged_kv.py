@@ -109,7 +109,8 @@ def paged_kv_plan(context_lens, query_lens, block_table, free_blocks, block_size
     ``context_lens``, ``query_lens`` int32 ``[N]``: tokens each request has in the cache and tokens it adds (0: it sits this
     step out).  ``block_table`` int32 ``[N, M]`` holds each request's pages; the entries of the pages this step opens are
     written, request by request, from ``free_blocks`` int32 ``[F]`` front to back (-1 once the list has run out).
-    ``num_tokens``: rows of the step's (possibly padded) batch.  ``state_rows`` int32 ``[N]``: each request's row in a state
+    ``num_tokens``: rows of the step's batch: padded, or cut off (tokens behind it get no slot; ``cu_seqlens`` and
+    ``seq_lens`` count them, so that the tokens before keep their places in their requests).  ``state_rows`` int32 ``[N]``: each request's row in a state
     pool.  Returns
 
     * ``slot_mapping`` int64 ``[num_tokens]``: page * block_size + offset, -1 for a token without a page and for padding,
@@ -229,8 +230,8 @@ def paged_kv_attention(query, key_cache, value_cache, key_scales, value_scales, 
     """Softmax attention over the cache: ``query [T, Hq, D]`` (bf16 or fp16; D 64, 128 or 256; Hq a multiple of the cache's
     heads), ``block_table`` int32 ``[N, M]``, ``seq_lens`` int32 ``[N]`` (tokens in the cache, the new ones included),
     ``cu_seqlens`` int32 ``[N + 1]`` the query rows of each request, or None for one row each (decode).  Row j of a
-    request's q rows is token ``seq_lens - q + j`` and sees the tokens up to itself; pages that the table gives a number
-    outside the pool are not seen, and a row that sees nothing is 0 with lse -inf.  ``scale`` defaults to ``D ** -0.5``.
+    request's q rows is token ``seq_lens - q + j`` and sees the tokens up to itself, also in a request that goes on behind the
+    last row of ``query``; pages that the table gives a number outside the pool are not seen, and a row that sees nothing is 0 with lse -inf.  ``scale`` defaults to ``D ** -0.5``.
     ``max_query_len``: the largest number of query rows of a request, if the caller knows it; it only chooses the kernel.
     Rows that belong to no request are 0 in a new result and left as they are in a given ``out``.  Returns ``out`` or, with
     ``return_lse``, ``(out, lse)`` with lse fp32 ``[T, Hq]`` (natural logarithm)."""

@@ -827,7 +827,8 @@ int fla_paged_kv_append(
 /* paged_kv_attention: out = softmax(scale * q k^T) v over the cached tokens of each request.  query, out [T,Hq,D] bf16
  * or f16 (D = 64, 128 or 256; Hq a multiple of the cache's heads); seq_lens i32 [N]: tokens in the cache, the new ones
  * included; cu_seqlens i32 [N+1]: the query rows of each request (NULL: one row for each request, T = N).  Query row j
- * of the q rows of request r is token seq_lens[r] - q + j and sees the tokens up to itself.  Pages that block_table
+ * of the q rows of request r is token seq_lens[r] - q + j and sees the tokens up to itself; q is what cu_seqlens says,
+ * also where T ends inside the request (a plan with fewer tokens than its requests add).  Pages that block_table
  * ([N,M] i32) gives a number outside the pool are not seen.  A row that sees nothing is 0 with lse -inf.  lse f32 [T,Hq]
  * optional: natural logarithm of the sum of exponentials.  max_query_len: the largest number of query rows of a request
  * (a hint that chooses the kernel; 0: unknown).  Rows that belong to no request (before cu_seqlens[0] or from

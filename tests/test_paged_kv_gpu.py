@@ -841,3 +841,43 @@ def test_rotary_gradient_has_a_gradient(dev, adjacent):
     assert all(torch.equal(a, b) for a, b in zip(grads, back)) and all(torch.equal(a, b) for a, b in zip(again, want))
     only = torch.autograd.grad(ops.rotary_axes(q, k, pos, freq, (6,), **how)[1], k, wk, create_graph=True)[0]
     assert torch.equal(torch.autograd.grad(only, wk, uk)[0], want[1])
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("new,kept", [(4, 2), (7, 9), (70, 33), (90, 100)])
+def test_requests_that_the_batch_cuts_off(dev, new, kept, wide):
+    """cu_seqlens past the rows of the query: a row keeps its place in its request, so it is as if the request were shorter by
+    the rows that are not there."""
+    from fla_hip import ops
+    rng, gen = random.Random(new), torch.Generator().manual_seed(new)
+    page, heads, kv_heads, dim, lens = 16, 8, 2, 64, [new + 40, new + 6, new + 300, new]
+    cu, rows = [new * r for r in range(5)], new + kept
+    kc, ks = random_cache(gen, 80, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, 80, kv_heads, page, dim, E4M3, dev)
+    table = make_table(rng, lens, page, max(-(-n // page) for n in lens), 80)
+    q = torch.randn(rows, heads, dim, generator=gen).to(BF)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    given = (widen(table, page) if wide else table).to(dev)
+    got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, given, i32(lens), i32(cu), max_query_len=new, return_lse=True)
+    cut = [min(c, rows) for c in cu]
+    short = [n - (new - (b - a)) for n, a, b in zip(lens, cut, cut[1:])]
+    check_attention(dev, q, (kc, vc, ks, vs), table, short, cut, dim ** -0.5, got=got)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("new,tokens", [(4, 6), (60, 100)])
+def test_a_step_with_fewer_rows_than_tokens(dev, new, tokens, wide):
+    """Plan, append and attention of a step whose batch ends inside a request: what is not appended (NaN here) is not seen."""
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(tokens)
+    page, heads, kv_heads, dim, n = 16, 4, 1, 64, 3
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    kc, vc = (torch.full((40, kv_heads, page, dim), 0x7f, dtype=torch.uint8, device=dev).view(E4M3) for _ in range(2))
+    ks, vs = torch.zeros(40, kv_heads, device=dev), torch.zeros(40, kv_heads, device=dev)
+    table = torch.full((n, 400 if wide else 12), -1, dtype=torch.int32, device=dev)
+    slots, _, cu, seq, _, _ = ops.paged_kv_plan(i32([0] * n), i32([new] * n), table, i32(list(range(39, 9, -1))), page, tokens)
+    q, k, v = (torch.randn(tokens, h, dim, generator=gen).to(BF) for h in (heads, kv_heads, kv_heads))
+    ops.paged_kv_append(k.to(dev), v.to(dev), kc, vc, ks, vs, slots)
+    got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, table, seq, cu, max_query_len=new, return_lse=True)
+    cut = [min(c, tokens) for c in cu.tolist()]
+    check_attention(dev, q, (kc, vc, ks, vs), table.cpu(), [b - a for a, b in zip(cut, cut[1:])], cut, dim ** -0.5, got=got)
