@@ -42,14 +42,15 @@ struct Request {
 
 __device__ __forceinline__ Request request_of(const AttnParams &p, int r) {
     Request q;
-    int a = r, b = r + 1;
+    int a = r, b = r + 1, all = r + 1;
     if (p.cu) {
         a = min(max(p.cu[r], 0), p.tokens);
-        b = min(max(p.cu[r + 1], a), p.tokens);
+        all = max(p.cu[r + 1], a);
+        b = min(all, p.tokens);
     }
     q.first = a;
     // Row j of a request is token len - (query tokens) + j also where q ends inside the request: the rows that q lacks count.
-    q.new_tokens = p.cu ? max(p.cu[r + 1], a) - a : 1;
+    q.new_tokens = all - a;
     q.rows = (b - a) * p.group;
     const int64_t most = (int64_t)p.width << p.shift;
     q.len = max(p.lens[r], 0);
