@@ -289,20 +289,24 @@ __device__ __forceinline__ float scale_unit(const AttnParams &p, const int32_t *
 //    contraction order of O^T.  V: lane 16 g + i loads D/16 neighbouring channels of those eight tokens, and a byte
 //    transpose inside the lane gives the operands of D/16 tiles whose row i is channel D/16 i + j of tile j.
 //  - scales of pages multiply S after the product (exact codes enter the matrix unit).  The v scale enters the weight of a
-//    token as an addend of its exponent, w = 2^(s + log2(vs / u) - m), which costs nothing for each element; m is the
+//    token as an addend of its exponent, w = 2^(s + log2(vs / u) - m), which costs nothing for each element; m is 10 below the
 //    largest s + log2(vs / u), so weights are measured against the largest contribution, whatever the scales of other
 //    pages are.  The sum of the softmax is that of w u / vs.  u, the scale of the request's first page as a power of two,
 //    only keeps these numbers inside fp32.  A scale below 2^-60 u (0 above all) counts as 2^-60 u in the exponent and
 //    multiplies the weight by the rest.
-//  - weights are rounded to fp16 with 11 bits: a bf16 weight would add an error as large as the rounding of the result.
-//  - the maximum moves only when the eight weights of a lane sum to more than 2^11 (fp16 holds 2^16), which the sum that is
-//    needed anyway tells, so most steps take no maximum, exchange nothing between lanes and rescale nothing.
+//  - weights are rounded to fp16 with 11 bits: a bf16 weight would add an error as large as the rounding of the result.  The
+//    largest contribution stands at 2^10 or more, near the top of fp16, because the sum of the softmax counts light weights in
+//    full: they keep 11 bits down to 2^-24 of the largest contribution and are off by at most 2^-35 of it below that, which
+//    shows only where a heavy token has values of (nearly) 0.
+//  - the maximum moves only when the eight weights of a lane sum to more than fp16 holds, which the sum that is needed anyway
+//    tells, so most steps take no maximum, exchange nothing between lanes and rescale nothing.  (Prefill of 2 x 4096 tokens: 788
+//    us with the largest contribution at 2^0 and sums to 2^11, 792 at 2^8 and 2^15, 804 at 2^10 and 2^15, 793 so.)
 // Sums and statistics are fp32.
 template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
     typedef elemx8 T8;
-    static constexpr float kMost = 0x1p11f;
+    static constexpr float kMost = 65504.f, kTop = 10.f;   // what sums may grow to, log2 of the weight of the largest contribution
     f32x4 o[NC][D / 16];   // o[c][j][e] of lane (g, i): channel D/16 (4 g + e) + j of query row 16 c + i, in units of u 2^m
-    float m[NC], l[NC];    // the largest s + log2(vs / u) when it last moved (the same in all lanes of a column), this lane's share of the sum
+    float m[NC], l[NC];    // the largest s + log2(vs / u) less kTop when it last moved (the same in all lanes of a column), this lane's share of the sum
     float unit, log_unit;  // u, log2 u
     unsigned seen;         // bit c: the column has seen a token
     bool fresh;
@@ -471,7 +475,7 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
         }
     }
 
-    // Moves the maximum of a column to its largest s + log2(vs / u) so far; `by`: what its sum and accumulators are to be
+    // Moves the maximum of a column to its largest s + log2(vs / u) so far, less kTop; `by`: what its sum and accumulators are to be
     // multiplied by.  A column that has seen nothing keeps a maximum of 0 (its scores are -inf, its weights 0).
     __device__ __forceinline__ void settle(const f32x4 (&s)[2], float f, float add, int c, float &by) {
         float best = kNegInf;
@@ -481,7 +485,7 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
             for (int e = 0; e < 4; ++e) best = fmaxf(best, s[t][e] * f);
         best += add;
         best = fmaxf(best, __shfl_xor(best, 16, kWave));
-        best = fmaxf(best, __shfl_xor(best, 32, kWave));
+        best = fmaxf(best, __shfl_xor(best, 32, kWave)) - kTop;
         const bool any = best > kNegInf, first = !(seen & (1u << c));
         const float top = !any ? m[c] : first ? best : fmaxf(best, m[c]);
         by = first ? 1.f : by * __builtin_amdgcn_exp2f(m[c] - top);                     // first: sum and accumulators are 0

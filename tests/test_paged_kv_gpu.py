@@ -881,3 +881,45 @@ def test_a_step_with_fewer_rows_than_tokens(dev, new, tokens, wide):
     got = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, table, seq, cu, max_query_len=new, return_lse=True)
     cut = [min(c, tokens) for c in cu.tolist()]
     check_attention(dev, q, (kc, vc, ks, vs), table.cpu(), [b - a for a, b in zip(cut, cut[1:])], cut, dim ** -0.5, got=got)
+
+
+@pytest.mark.parametrize("gap", [14.0, 17.0, 18.0, 20.0])
+@pytest.mark.parametrize("rows,heads,n", [(2340, 64, 4096), (40, 4, 250), (1, 4, 1500)])
+def test_a_first_token_that_draws_the_weight_and_holds_no_values(dev, rows, heads, n, gap):
+    """The first key of a text stands ``gap`` nats above the others and its values are 0, so the result is what the light weights
+    add up to.  A weight is fp16 with the largest contribution at 2^10 or more: one below 2^-14 is off by at most 2^-25, so
+    2^-35 of the largest contribution, times its code.  In float64 on the GPU, some heads."""
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(int(gap))
+    page, dim = 64, 64
+    pool = -(-n // page)
+    k = torch.randn(pool, heads, page, dim, generator=gen) * 0.25
+    k[..., 0] = 0
+    k[0, :, 0] = 0
+    k[0, :, 0, 0] = 16.0
+    v = torch.rand(pool, heads, page, dim, generator=gen) * 3 + 1
+    v[0, :, 0] = 0
+    kc, vc = k.to(E4M3).to(dev), v.to(E4M3).to(dev)
+    ones = torch.ones(pool, heads, device=dev)
+    q = torch.randn(rows, heads, dim, generator=gen) * 0.5
+    scale = 0.125
+    q[..., 0] = gap / 16 / scale
+    q = q.to(BF).to(dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    out, lse = ops.paged_kv_attention(q, kc, vc, ones, ones, torch.arange(pool, device=dev, dtype=torch.int32)[None], i32([n]), i32([0, rows]),
+                                      scale=scale, max_query_len=rows, return_lse=True)
+    seen = torch.arange(n, device=dev) <= torch.arange(n - rows, n, device=dev)[:, None]
+    for h in range(0, heads, max(1, heads // 4)):
+        kd, vd = (c.view(torch.uint8)[:, h].view(E4M3).float().double().flatten(0, 1)[:n] for c in (kc, vc))
+        x = q[:, h].double()
+        score = torch.where(seen, (x @ kd.t()) * scale, -math.inf)
+        p = torch.softmax(score, -1)
+        want = p @ vd
+        err = (dim + 8) * 2.0 ** -24 * ((x.abs() @ kd.abs().t()) * scale).amax(-1)[:, None]
+        peak = p.amax(-1)[:, None]
+        # the result's rounding (8 significant bits: 2^-8 of its value), the weights' (2^-12) and the scores'; codes are at most 4
+        bound = want * (torch.finfo(BF).eps / 2 * 1.01 + 2.0 ** -12 * 1.01 + 2 * err) + n * 2.0 ** -35 * peak * 4 + torch.finfo(BF).tiny
+        error = (out[:, h].double() - want).abs()
+        assert bool((error <= bound).all()), (h, float((error / bound).max()), float((error / want).max()))
+        want_lse = score.logsumexp(-1)
+        assert bool(((lse[:, h].double() - want_lse).abs() <= err[:, 0] + 2.0 ** -21 * (1 + want_lse.abs())).all())
