@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(W * 64) paged_kv_append_kernel(const AppendPar
         }
         // a power of two (every scale this operator writes): an exact product; another scale from outside: a division
         const bool exact = (__builtin_bit_cast(unsigned, after) & 0x7fffffu) == 0;
-        const float inv = after > 0.f ? 1.f / after : 0.f;
+        const float inv = after > 0.f ? 1.f / after : 1.f;                        // scale 0: zeros, and what is not finite as it is
         const bool plain = exact && !__any(odd);
 #pragma unroll
         for (int m = 0; m < kHeld; ++m) {

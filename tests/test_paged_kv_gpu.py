@@ -923,3 +923,27 @@ def test_a_first_token_that_draws_the_weight_and_holds_no_values(dev, rows, head
         assert bool((error <= bound).all()), (h, float((error / bound).max()), float((error / want).max()))
         want_lse = score.logsumexp(-1)
         assert bool(((lse[:, h].double() - want_lse).abs() <= err[:, 0] + 2.0 ** -21 * (1 + want_lse.abs())).all())
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_append_of_infinities_without_a_finite_value(dev, code, dtype):
+    """Pages whose scale is 0: infinities store the largest code all the same, NaN stores NaN (e4m3) or 0 (int8)."""
+    from fla_hip import ops
+    page, dim, heads = 16, 64, 2
+    x = torch.zeros(6, heads, dim, dtype=dtype)
+    x[0, 0, 3], x[0, 0, 5], x[1, 1, 7], x[2, 0, 9] = math.inf, -math.inf, math.nan, math.inf
+    x[4, 0, 0], x[5, 0, 0] = math.inf, 1.0                               # a finite row later on
+    slots = [0, 1, page, 2 * page + 15, 3 * page, 3 * page + 1]
+    new = lambda: torch.zeros(5, heads, page, dim, dtype=torch.uint8, device=dev).view(code)
+    kc, vc, ks, vs = new(), new(), torch.full((5, heads), 3.0, device=dev), torch.full((5, heads), 3.0, device=dev)
+    want, scale = torch.zeros(5, heads, page, dim, dtype=torch.float64), torch.full((5, heads), 3.0, dtype=torch.float64)
+    ks[2], scale[2] = 0, 0
+    vs[2] = 0
+    for part in (slice(0, 5), slice(5, 6)):
+        ops.paged_kv_append(x[part].to(dev), -x[part].to(dev), kc, vc, ks, vs, torch.tensor(slots[part], device=dev))
+        ref.append(x[part], want, scale, slots[part], code)
+        assert torch.equal(ks.cpu().double(), scale) and torch.equal(vs.cpu().double(), scale)
+        for cache, sign in ((kc, 1), (vc, -1)):
+            got = codes_of(cache) * sign
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
