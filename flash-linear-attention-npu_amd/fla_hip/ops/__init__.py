@@ -141,6 +141,14 @@ def _has_tensor_requiring_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
+def _has_tangent(*tensors) -> bool:
+    """Whether one of the tensors (or None) is a dual tensor of forward-mode differentiation."""
+    import torch
+
+    ad = torch.autograd.forward_ad
+    return ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def causal_conv1d(x, weight, bias=None, conv_states=None, *, query_start_loc=None, cache_indices=None,
                   initial_state_mode=None, num_accepted_tokens=None, activation_mode=0, pad_slot_id=-1,
                   run_mode=0, head_num=0):
@@ -192,30 +200,47 @@ def _rotary_function():
     import torch
 
     class RotaryAxes(torch.autograd.Function):
-        """Linear in q and k: the gradient is the inverse turn, which is an operator of the same kind."""
+        """Linear in q and k: the tangent is the same turn, the gradient the inverse one, which is an operator of the same kind."""
 
         @staticmethod
         def forward(ctx, q, k, positions, inv_freq, sections, axis_order, pairing, inverse):
             ctx.save_for_backward(positions, inv_freq)
+            ctx.save_for_forward(positions, inv_freq)
             ctx.how = sections, axis_order, pairing, not inverse
             ctx.set_materialize_grads(False)
             return _paged_kv._rotate(q, k, positions, inv_freq, sections, axis_order, pairing, inverse)
 
         @staticmethod
         def backward(ctx, dq, dk):
-            turn = RotaryAxes.apply if torch.is_grad_enabled() else _paged_kv._rotate      # enabled: a graph of the gradient is wanted
-            dq, dk = [g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk)]
-            if dq is not None:
-                dq, dk = turn(dq, dk, *ctx.saved_tensors, *ctx.how)
-            elif dk is not None:
-                dk = turn(dk, None, *ctx.saved_tensors, *ctx.how)[0]
-            return dq, dk, None, None, None, None, None, None
+            return *_rotary(RotaryAxes.rows(dq), RotaryAxes.rows(dk), *ctx.saved_tensors, *ctx.how), None, None, None, None, None, None
+
+        @staticmethod
+        def jvp(ctx, tq, tk, *rest):
+            *how, inverse = ctx.how
+            return _rotary(RotaryAxes.rows(tq), RotaryAxes.rows(tk), *ctx.saved_tensors, *how, not inverse)
+
+        @staticmethod
+        def rows(x):
+            return x if x is None or x.stride(-1) == 1 else x.contiguous()
 
     return RotaryAxes
 
 
+def _rotary(q, k, *how):
+    """The turn of q and k (either may be None), through autograd where a derivative is wanted."""
+    if q is None:
+        return None, None if k is None else _rotary(k, None, *how)[0]
+    if _has_tangent(q, k):
+        if k is not None:                                  # one by one: a result of the autograd function has a tangent or is None
+            return _rotary(q, None, *how)[0], _rotary(k, None, *how)[0]
+    elif not _has_tensor_requiring_grad(q, k):
+        return _paged_kv._rotate(q, k, *how)
+    return _rotary_function().apply(q, k, *how)
+
+
 def rotary_axes(q, k, positions, inv_freq, sections, *, axis_order="blocked", pairing="half"):
-    """Rotary positions with one or more axes (text; height and width; time, height and width), differentiable in q and k.
+    """Rotary positions with one or more axes (text; height and width; time, height and width), differentiable in q and k
+    (backward and forward mode, any number of times).
 
     ``q``, ``k`` (or None) ``[B, T, H, D]`` or ``[T, H, D]`` in bf16, fp16 or fp32, with any outer strides and numbers of heads of
     their own; ``positions`` int32 or int64 ``[axes, B, T]`` or ``[axes, T]``; ``inv_freq`` fp32 ``[R / 2]`` on the device;
@@ -224,9 +249,9 @@ def rotary_axes(q, k, positions, inv_freq, sections, *, axis_order="blocked", pa
     (formed in 64 bits); a pair is channels j and j + R/2 (``pairing="half"``) or 2j and 2j + 1 (``"adjacent"``).  Channels
     from R on pass through.  Returns the rotated q and k in the memory order of the inputs."""
     _paged_kv._refuse_grad("rotary_axes", inv_freq=inv_freq)
-    if _has_tensor_requiring_grad(q, k):
-        return _rotary_function().apply(q, k, positions, inv_freq, sections, axis_order, pairing, False)
-    return _paged_kv._rotate(q, k, positions, inv_freq, sections, axis_order, pairing, False)
+    if q is None:
+        raise TypeError("rotary_axes: q must be a tensor; a single operand is passed as q.")
+    return _rotary(q, k, positions, inv_freq, sections, axis_order, pairing, False)
 
 
 __all__ = [

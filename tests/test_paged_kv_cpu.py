@@ -354,3 +354,52 @@ def test_rotary_refuses_frequencies_that_want_a_gradient():
     q, freq = torch.zeros(5, 2, 16, dtype=torch.bfloat16), torch.ones(4, requires_grad=True)
     with pytest.raises(NotImplementedError, match="no gradient is bound for inv_freq"):
         ops.rotary_axes(q, None, torch.zeros(1, 5, dtype=torch.int64), freq, (4,))
+
+
+@pytest.fixture
+def plain_rotary(monkeypatch):
+    """``rotary_axes`` with the oracle in the place of the launch."""
+    from fla_hip.ops import _paged_kv as P
+
+    def rotate(q, k, positions, inv_freq, sections, axis_order, pairing, inverse):
+        assert q.stride(-1) == 1
+        return tuple(None if x is None else ref.rotary(x.detach(), positions, inv_freq, sections, axis_order, pairing, inverse).to(x.dtype) for x in (q, k))
+
+    monkeypatch.setattr(P, "_rotate", rotate)
+
+
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+def test_rotary_has_a_tangent(plain_rotary, pairing):
+    """Linear in q and k: the tangent is the operator applied to the tangents.  Also under a reverse pass, in its gradient, and where
+    only one of q and k has one."""
+    from fla_hip import ops
+    from torch.autograd import forward_ad as ad
+
+    gen = torch.Generator().manual_seed(3)
+    q, tq, wq = (torch.randn(5, 3, 12, generator=gen, dtype=torch.float64) for _ in range(3))
+    k, tk, wk = (torch.randn(5, 1, 12, generator=gen, dtype=torch.float64) for _ in range(3))
+    pos, freq = torch.randint(0, 50, (2, 5), generator=gen), torch.rand(4, generator=gen)
+    turn = lambda a, b=None: ops.rotary_axes(a, b, pos, freq, (3, 1), pairing=pairing)
+    back = lambda x: ref.rotary(x, pos, freq, (3, 1), "blocked", pairing, True)
+    want = turn(tq, tk)
+    tangent = lambda x: ad.unpack_dual(x).tangent
+    with ad.dual_level():
+        a, b = turn(ad.make_dual(q, tq), ad.make_dual(k, tk))
+        assert torch.equal(tangent(a), want[0]) and torch.equal(tangent(b), want[1]) and torch.equal(ad.unpack_dual(a).primal, turn(q)[0])
+        a, b = turn(ad.make_dual(q, tq), k)
+        assert torch.equal(tangent(a), want[0]) and (tangent(b) is None or not bool(tangent(b).any()))
+        a, b = turn(q, ad.make_dual(k, tk))
+        assert torch.equal(tangent(b), want[1]) and (tangent(a) is None or not bool(tangent(a).any()))
+        a, none = turn(ad.make_dual(q, tq))
+        assert none is None and torch.equal(tangent(a), want[0])
+        with torch.no_grad():
+            assert torch.equal(tangent(turn(ad.make_dual(q, tq))[0]), want[0])
+        leaf, direction = q.clone().requires_grad_(), tq.clone().requires_grad_()      # both modes at once
+        a, _ = turn(ad.make_dual(leaf, direction))
+        assert torch.equal(tangent(a), want[0])
+        assert torch.equal(torch.autograd.grad(tangent(a), direction, wq, retain_graph=True)[0], back(wq))
+        got = torch.autograd.grad(a, leaf, ad.make_dual(wq, tq))[0]                    # the gradient has a tangent too
+        assert torch.equal(ad.unpack_dual(got).primal, back(wq)) and torch.equal(tangent(got), back(tq))
+    got = torch.autograd.grad(turn(leaf, k.requires_grad_()), (leaf, k), (wq, wk.expand_as(k)))
+    assert torch.equal(got[0], back(wq)) and torch.equal(got[1], back(wk))
+    assert torch.autograd.gradcheck(lambda x, y: turn(x, y), (leaf, k), check_forward_ad=True)

@@ -947,3 +947,22 @@ def test_append_of_infinities_without_a_finite_value(dev, code, dtype):
         for cache, sign in ((kc, 1), (vc, -1)):
             got = codes_of(cache) * sign
             assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+def test_rotary_has_a_tangent(dev):
+    """The same kernel on the tangents: equal to the bit, in the gradient as well; expanded tangents among them."""
+    from fla_hip import ops
+    from torch.autograd import forward_ad as ad
+    gen = torch.Generator().manual_seed(4)
+    q, tq, w = (torch.randn(9, 3, 16, generator=gen).to(dev) for _ in range(3))
+    k, tk = torch.randn(9, 1, 16, generator=gen).to(dev), torch.randn(9, 1, 1, generator=gen).to(dev).expand(9, 1, 16)
+    how = torch.arange(9, device=dev)[None], torch.rand(6, generator=gen).to(dev), (6,)
+    want = ops.rotary_axes(q, k, *how) + ops.rotary_axes(tq, tk.contiguous(), *how)
+    with ad.dual_level():
+        leaf = q.clone().requires_grad_()
+        for x in (q, leaf):
+            y = ops.rotary_axes(ad.make_dual(x, tq), ad.make_dual(k, tk), *how)
+            got = [ad.unpack_dual(a) for a in y]
+            assert all(torch.equal(a, b) for a, b in zip([g.primal for g in got] + [g.tangent for g in got], want))
+        dq = ad.unpack_dual(torch.autograd.grad(y[0], leaf, ad.make_dual(w, tq))[0])
+        assert torch.equal(dq.primal, ops.rotary_axes_bwd(w, None, *how)[0]) and torch.equal(dq.tangent, ops.rotary_axes_bwd(tq, None, *how)[0])
