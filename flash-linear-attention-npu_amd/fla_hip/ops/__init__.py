@@ -141,14 +141,6 @@ def _has_tensor_requiring_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
-def _has_tangent(*tensors) -> bool:
-    """Whether one of the tensors (or None) is a dual tensor of forward-mode differentiation."""
-    import torch
-
-    ad = torch.autograd.forward_ad
-    return ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors)
-
-
 def causal_conv1d(x, weight, bias=None, conv_states=None, *, query_start_loc=None, cache_indices=None,
                   initial_state_mode=None, num_accepted_tokens=None, activation_mode=0, pad_slot_id=-1,
                   run_mode=0, head_num=0):
@@ -230,7 +222,7 @@ def _rotary(q, k, *how):
     """The turn of q and k (either may be None), through autograd where a derivative is wanted."""
     if q is None:
         return None, None if k is None else _rotary(k, None, *how)[0]
-    if _has_tangent(q, k):
+    if _paged_kv.has_tangent(q, k):
         if k is not None:                                  # one by one: a result of the autograd function has a tangent or is None
             return _rotary(q, None, *how)[0], _rotary(k, None, *how)[0]
     elif not _has_tensor_requiring_grad(q, k):

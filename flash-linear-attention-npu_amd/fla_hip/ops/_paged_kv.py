@@ -94,13 +94,22 @@ class _Call:
             raise RuntimeError(f"fla_{name} failed with status={status}: {_runtime.last_error()}")
 
 
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors (or None) is a dual tensor of forward-mode differentiation."""
+    import torch
+
+    ad = torch.autograd.forward_ad
+    return ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _refuse_grad(op: str, **tensors):
     import torch
 
-    if torch.is_grad_enabled():
-        needing = [name for name, t in tensors.items() if t.requires_grad]
-        if needing:
-            raise NotImplementedError(f"fla_hip.ops.{op}: no gradient is bound for {', '.join(needing)}; pass detached tensors.")
+    needing = [name for name, t in tensors.items() if getattr(t, "requires_grad", False)] if torch.is_grad_enabled() else []
+    if torch.autograd.forward_ad._current_level >= 0:
+        needing += [name for name, t in tensors.items() if name not in needing and has_tangent(t)]
+    if needing:
+        raise NotImplementedError(f"fla_hip.ops.{op}: no gradient is bound for {', '.join(needing)}; pass detached tensors.")
 
 
 def paged_kv_plan(context_lens, query_lens, block_table, free_blocks, block_size: int, num_tokens: int, *, state_rows=None):
@@ -214,8 +223,8 @@ def paged_kv_append(key, value, key_cache, value_cache, key_scales, value_scales
     two ``s`` with ``max|x| / s <= 448`` (e4m3) or ``127`` (int8) over the tokens of that page and head so far; when it grows,
     the codes already there are converted.  Tokens of a page before the first new one are kept; a page whose offset 0 is
     written starts afresh.  Infinities store the largest code; NaN stores NaN (e4m3) or 0 (int8)."""
+    _refuse_grad("paged_kv_append", key=key, value=value, key_scales=key_scales, value_scales=value_scales)
     call = _Call(key_cache, "key_cache")
-    _refuse_grad("paged_kv_append", key=key, value=value)
     if key.dim() != 3 or key.shape[0] == 0:
         if key.dim() == 3 and key.shape == value.shape and slot_mapping.numel() == 0:
             return
@@ -237,8 +246,8 @@ def paged_kv_attention(query, key_cache, value_cache, key_scales, value_scales, 
     ``return_lse``, ``(out, lse)`` with lse fp32 ``[T, Hq]`` (natural logarithm)."""
     import torch
 
+    _refuse_grad("paged_kv_attention", query=query, key_cache=key_cache, value_cache=value_cache, key_scales=key_scales, value_scales=value_scales)
     call = _Call(query, "query")
-    _refuse_grad("paged_kv_attention", query=query)
     if query.dim() != 3:
         raise ValueError(f"paged_kv_attention: query must be [T, Hq, D], got rank {query.dim()}.")
     clear = out is None

@@ -403,3 +403,31 @@ def test_rotary_has_a_tangent(plain_rotary, pairing):
     got = torch.autograd.grad(turn(leaf, k.requires_grad_()), (leaf, k), (wq, wk.expand_as(k)))
     assert torch.equal(got[0], back(wq)) and torch.equal(got[1], back(wk))
     assert torch.autograd.gradcheck(lambda x, y: turn(x, y), (leaf, k), check_forward_ad=True)
+
+
+def test_derivatives_that_are_not_bound_are_refused():
+    """Whatever enters the result: queries, caches, scales, frequencies; by gradient and by tangent."""
+    from fla_hip import ops
+    from torch.autograd import forward_ad as ad
+
+    x, i = torch.zeros(2, 1, 64), torch.zeros(2, dtype=torch.int32)
+    cache, scale = torch.zeros(2, 1, 16, 64).to(torch.float8_e4m3fn), torch.zeros(2, 1)
+    attention = dict(query=x, key_cache=cache, value_cache=cache, key_scales=scale, value_scales=scale)
+    append = dict(key=x, value=x, key_cache=cache, value_cache=cache, key_scales=scale, value_scales=scale)
+    for name in attention:
+        changed = attention | {name: attention[name].clone().requires_grad_()}
+        with pytest.raises(NotImplementedError, match=f"paged_kv_attention: no gradient is bound for {name}"):
+            ops.paged_kv_attention(**changed, block_table=i[:, None], seq_lens=i)
+        with torch.no_grad(), pytest.raises(TypeError, match="ROCm GPU tensor"):       # no derivative is asked for
+            ops.paged_kv_attention(**changed, block_table=i[:, None], seq_lens=i)
+    for name in ("key", "value"):
+        with pytest.raises(NotImplementedError, match=f"paged_kv_append: no gradient is bound for {name}"):
+            ops.paged_kv_append(**append | {name: x.clone().requires_grad_()}, slot_mapping=i.long())
+    with ad.dual_level():
+        for op, args, rest in ((ops.paged_kv_attention, attention, dict(block_table=i[:, None], seq_lens=i)), (ops.paged_kv_append, append, dict(slot_mapping=i.long()))):
+            for name in args:
+                if not name.endswith("cache"):
+                    with pytest.raises(NotImplementedError, match=f"no gradient is bound for {name}"), torch.no_grad():
+                        op(**args | {name: ad.make_dual(args[name], torch.ones_like(args[name]))}, **rest)
+        with pytest.raises(NotImplementedError, match="no gradient is bound for inv_freq"):
+            ops.rotary_axes(x, None, i[None], ad.make_dual(torch.ones(4), torch.ones(4)), (4,))
