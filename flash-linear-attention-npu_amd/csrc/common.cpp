@@ -41,6 +41,24 @@ bool same_shape(const fla_tensor *a, const fla_tensor *b) {
     return true;
 }
 
+bool separate(const fla_tensor *t) {
+    int order[FLA_MAX_DIMS], n = 0;
+    for (int i = 0; i < t->ndim; ++i) {
+        if (t->shape[i] == 0) return true;
+        if (t->shape[i] == 1) continue;
+        int at = n++;
+        for (; at > 0 && t->stride[order[at - 1]] > t->stride[i]; --at) order[at] = order[at - 1];
+        order[at] = i;
+    }
+    int64_t reach = 1;                 // elements from the first to the last of the dimensions so far
+    for (int k = 0; k < n; ++k) {
+        const int64_t stride = t->stride[order[k]], extent = t->shape[order[k]];
+        if (stride < reach || stride > (INT64_MAX - reach) / extent) return false;
+        reach += stride * (extent - 1);
+    }
+    return true;
+}
+
 int build_varlen(Varlen &vl, const char *op, const fla_int_array *cu, const fla_int_array *ci,
                  int64_t chunk, int64_t total_t) {
     vl = Varlen();

@@ -76,6 +76,9 @@ inline int64_t numel(const fla_tensor *t) {
 int check_tensor(const fla_tensor *t, const char *op, const char *name, int ndim, int dtype_mask);
 inline int dt_bit(int dt) { return 1 << dt; }
 bool same_shape(const fla_tensor *a, const fla_tensor *b);
+// No two elements share memory: sorted by stride, each dimension steps over all that the smaller ones reach.  Layouts that do
+// not nest like that count as overlapping.
+bool separate(const fla_tensor *t);
 // Innermost stride must be 1 (or extent 1).
 inline bool inner_unit(const fla_tensor *t) {
     return t->ndim == 0 || t->shape[t->ndim - 1] == 1 || t->stride[t->ndim - 1] == 1;

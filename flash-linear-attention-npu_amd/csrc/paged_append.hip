@@ -274,10 +274,8 @@ int append_impl(const fla_tensor *key, const fla_tensor *value, const fla_tensor
         FLA_REQUIRE(inner_unit(x[i]) && x[i]->stride[0] >= 0 && x[i]->stride[1] >= 0 && x[i]->stride[0] % 8 == 0 && x[i]->stride[1] % 8 == 0 &&
                         reinterpret_cast<uintptr_t>(x[i]->data) % 16 == 0,
                     FLA_ERR_SHAPE, "%s: rows of %s must be contiguous and 16-byte aligned.", op, i ? "value" : "key");
-        for (int d = 0; d < 3; ++d)
-            FLA_REQUIRE(cache[i]->shape[d] == 1 || cache[i]->stride[d] > 0, FLA_ERR_SHAPE, "%s: rows of %s overlap.", op, i ? "value_cache" : "key_cache");
-        for (int d = 0; d < 2; ++d)
-            FLA_REQUIRE(scales[i]->shape[d] == 1 || scales[i]->stride[d] > 0, FLA_ERR_SHAPE, "%s: elements of %s overlap.", op, i ? "value_scales" : "key_scales");
+        FLA_REQUIRE(separate(cache[i]), FLA_ERR_SHAPE, "%s: rows of %s overlap.", op, i ? "value_cache" : "key_cache");
+        FLA_REQUIRE(separate(scales[i]), FLA_ERR_SHAPE, "%s: elements of %s overlap.", op, i ? "value_scales" : "key_scales");
         // rows of a page are addressed with 32-bit offsets
         FLA_REQUIRE(x[i]->stride[0] < ((int64_t)1 << 21) && cache[i]->stride[2] < ((int64_t)1 << 23), FLA_ERR_UNSUPPORTED,
                     "%s: tokens of %s or its cache lie too far apart.", op, i ? "value" : "key");
@@ -303,6 +301,8 @@ int append_impl(const fla_tensor *key, const fla_tensor *value, const fla_tensor
     p.dim = (int)shape.dim;
     if (p.tokens == 0) return FLA_OK;
     FLA_REQUIRE(p.tokens < ((int64_t)1 << 26), FLA_ERR_SHAPE, "%s: too many tokens.", op);
+    FLA_REQUIRE(key_cache->data != value_cache->data && key_scales->data != value_scales->data, FLA_ERR_SHAPE,
+                "%s: keys and values need caches and scales of their own.", op);
     p.row_shift = __builtin_ctz((unsigned)p.dim / 8);
 #define FLA_BY_TYPE(CODE)                                                                \
     (key->dtype == FLA_BF16 ? launch<bf16, CODE>(p, stream) : key->dtype == FLA_F16 ? launch<f16, CODE>(p, stream) : launch<float, CODE>(p, stream))

@@ -27,7 +27,7 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
                         reinterpret_cast<uintptr_t>(t->data) % 16 == 0,
                     FLA_ERR_SHAPE, "%s: rows of %s must be contiguous and 16-byte aligned.", op, t == q ? "query" : "out");
     }
-    FLA_REQUIRE((out->stride[0] > 0 || T <= 1) && (out->stride[1] > 0 || heads <= 1), FLA_ERR_SHAPE, "%s: rows of out overlap.", op);
+    FLA_REQUIRE(separate(out), FLA_ERR_SHAPE, "%s: rows of out overlap.", op);
     if ((rc = check_tensor(table, op, "block_table", 2, dt_bit(FLA_I32)))) return rc;
     if ((rc = check_tensor(lens, op, "seq_lens", 1, dt_bit(FLA_I32)))) return rc;
     const int64_t n = table->shape[0];
@@ -42,6 +42,7 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
     if (present(lse)) {
         if ((rc = check_tensor(lse, op, "lse", 2, dt_bit(FLA_F32)))) return rc;
         FLA_REQUIRE(lse->shape[0] == T && lse->shape[1] == heads && lse->stride[0] >= 0 && lse->stride[1] >= 0, FLA_ERR_SHAPE, "%s: lse must be [T,Hq].", op);
+        FLA_REQUIRE(separate(lse), FLA_ERR_SHAPE, "%s: elements of lse overlap.", op);
     }
     const int64_t group = heads / shape.heads;
     FLA_REQUIRE(T * group < ((int64_t)1 << 31) && n < ((int64_t)1 << 24) && table->shape[1] < ((int64_t)1 << 31), FLA_ERR_SHAPE, "%s: sizes exceed the supported range.", op);

@@ -135,10 +135,10 @@ int rows_of(const char *op, const char *name, const fla_tensor *x, const fla_ten
     int64_t all = (int64_t)(reinterpret_cast<uintptr_t>(x->data) | reinterpret_cast<uintptr_t>(y->data));
     for (int i = 0; i < x->ndim - 1; ++i) {
         FLA_REQUIRE(x->stride[i] >= 0 && y->stride[i] >= 0, FLA_ERR_SHAPE, "%s: negative strides are not supported.", op);
-        FLA_REQUIRE(y->shape[i] <= 1 || y->stride[i] > 0, FLA_ERR_SHAPE, "%s: rows of an output overlap.", op);
         if (x->shape[i] > 1) all |= x->stride[i] * size;
         if (y->shape[i] > 1) all |= y->stride[i] * size;
     }
+    FLA_REQUIRE(separate(y), FLA_ERR_SHAPE, "%s: rows of an output overlap.", op);
     while (piece > 1 && all % (piece * size)) piece >>= 1;
     return FLA_OK;
 }

@@ -819,7 +819,8 @@ int fla_rotary_axes(
  * A page's scale is the smallest power of two s (at least 2^-126) with max|x| / s <= 448 (e4m3) or 127 (int8) over the
  * finite elements stored so far in that page and head, 0 while all are 0; when it grows, the codes already there are
  * converted to it.  Codes are x / s rounded to nearest even; infinities store the largest code, NaN stores NaN (e4m3)
- * or 0 (int8).  Rows of the caches and elements of the scales must not overlap; T < 2^26. */
+ * or 0 (int8).  Keys and values have caches and scales of their own, in which no two elements share memory (a layout whose
+ * strides do not nest, each stepping over all that the smaller ones reach, is refused); T < 2^26. */
 int fla_paged_kv_append(
     const fla_tensor *key, const fla_tensor *value, const fla_tensor *key_cache, const fla_tensor *value_cache,
     const fla_tensor *key_scales, const fla_tensor *value_scales, const fla_tensor *slot_mapping, void *stream);

@@ -431,3 +431,44 @@ def test_derivatives_that_are_not_bound_are_refused():
                         op(**args | {name: ad.make_dual(args[name], torch.ones_like(args[name]))}, **rest)
         with pytest.raises(NotImplementedError, match="no gradient is bound for inv_freq"):
             ops.rotary_axes(x, None, i[None], ad.make_dual(torch.ones(4), torch.ones(4)), (4,))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(kc=desc((10, 2, 16, 128), I8, (2048, 2048, 128, 1))), "rows of key_cache overlap"),        # pages one head apart
+    (dict(vc=desc((10, 2, 16, 128), I8, (4096, 2048, 64, 1))), "rows of value_cache overlap"),       # tokens half a row apart
+    (dict(kc=desc((10, 2, 16, 128), I8, (4096, 16, 128, 1))), "rows of key_cache overlap"),
+    (dict(kc=desc((10, 2, 16, 128), I8, (2032, 1 << 20, 128, 1))), "rows of key_cache overlap"),     # the last row of a page is the next one's
+    (dict(ks=desc((10, 2), F32, (1, 1))), "elements of key_scales overlap"),
+    (dict(vs=desc((10, 2), F32, (1, 9))), "elements of value_scales overlap"),
+    (dict(vc=desc((10, 2, 16, 128), I8, data=4096)), "caches and scales of their own"),
+    (dict(ks=desc((10, 2), F32, data=8192), vs=desc((10, 2), F32, data=8192), vc=desc((10, 2, 16, 128), I8, data=1 << 20)), "caches and scales of their own"),
+])
+def test_append_refuses_memory_that_two_rows_share(lib, change, text):
+    """Two workgroups would write it in no order; nothing is launched."""
+    from fla_hip.ops import _paged_kv as P
+
+    fn = lib.fla_paged_kv_append
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["paged_kv_append"], ctypes.c_void_p], ctypes.c_int
+    assert fn(*append_args(**change), None) == SHAPE and text in lib.fla_last_error().decode(), lib.fla_last_error()
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(out=desc((6, 8, 128), BF16, (128, 128, 1))), "rows of out overlap"),
+    (dict(out=desc((6, 8, 128), BF16, (1024, 64, 1))), "rows of out overlap"),
+    (dict(lse=desc((6, 8), F32, (0, 1))), "elements of lse overlap"),
+    (dict(lse=desc((6, 8), F32, (7, 1))), "elements of lse overlap"),
+])
+def test_attention_refuses_results_that_two_rows_share(lib, change, text):
+    assert query(lib, attention_args(**change))[0] == SHAPE and text in lib.fla_last_error().decode()
+    nested = dict(out=desc((6, 8, 128), BF16, (128, 1024, 1)), lse=desc((6, 8), F32, (1, 6)))       # heads first: nothing shared
+    assert query(lib, attention_args(**nested))[0] == OK
+
+
+def test_rotary_refuses_results_that_two_rows_share(lib):
+    from fla_hip.ops import _paged_kv as P
+
+    fn = lib.fla_rotary_axes
+    fn.argtypes, fn.restype = [*P.OP_ARGTYPES["rotary_axes"], ctypes.c_void_p], ctypes.c_int
+    for out in (dict(q_out=desc((5, 2, 16), BF16, (16, 16, 1))), dict(k_out=desc((5, 1, 16), BF16, (8, 16, 1)))):
+        args, keep = rotary_args(**out)
+        assert fn(*args, None) == SHAPE and "rows of an output overlap" in lib.fla_last_error().decode()
