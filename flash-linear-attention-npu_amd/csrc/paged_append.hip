@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(W * 64) paged_kv_append_kernel(const AppendPar
 #pragma unroll
             for (int w = 0; w < W; ++w) most = fmaxf(most, wave_max[w]);
         }
-        const float after = fmaxf(before, step_for<CODE>(most));
+        const float after = fmaxf(fabsf(before), step_for<CODE>(most));           // a negative scale comes from outside
         uint8_t *cache = static_cast<uint8_t *>(s.cache) + block * s.c_p + head * s.c_h;
         if (after > before) {
             const float ratio = before / after;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(W * 64) paged_kv_append_kernel(const AppendPar
                     float v[4];
                     decode4<CODE>(code[w], v);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] *= ratio;
+                    for (int e = 0; e < 4; ++e) v[e] = CODE == FLA_I8 ? fminf(v[e] * ratio, 127.f) : v[e] * ratio;   // -128 times -1
                     code[w] = encode4<CODE>(v);
                 }
                 *to = code;

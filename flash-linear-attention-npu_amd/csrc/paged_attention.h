@@ -275,7 +275,7 @@ template <int D, bool WIDE, Loads L> struct ValueCodes {
 // The power of two that the v scales of a request and head are measured in: that of its first page, if it has one.
 __device__ __forceinline__ float scale_unit(const AttnParams &p, const int32_t *table_row, int head) {
     const int page = p.width ? table_row[0] : -1;
-    const float s = (uint32_t)page < p.pool ? p.vs[(int64_t)page * p.vs_p + head * p.vs_h] : 0.f;
+    const float s = (uint32_t)page < p.pool ? fabsf(p.vs[(int64_t)page * p.vs_p + head * p.vs_h]) : 0.f;
     if (!(s > 0.f && s < INFINITY)) return 0x1p-40f;
     return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, fminf(fmaxf(s, 0x1p-60f), 0x1p60f)) & 0x7f800000u);
 }
@@ -293,7 +293,7 @@ __device__ __forceinline__ float scale_unit(const AttnParams &p, const int32_t *
 //    largest s + log2(vs / u), so weights are measured against the largest contribution, whatever the scales of other
 //    pages are.  The sum of the softmax is that of w u / vs.  u, the scale of the request's first page as a power of two,
 //    only keeps these numbers inside fp32.  A scale below 2^-60 u (0 above all) counts as 2^-60 u in the exponent and
-//    multiplies the weight by the rest.
+//    multiplies the weight by the rest; of a negative one the magnitude is in the exponent.
 //  - weights are rounded to fp16 with 11 bits: a bf16 weight would add an error as large as the rounding of the result.  The
 //    largest contribution stands at 2^10 or more, near the top of fp16, because the sum of the softmax counts light weights in
 //    full: they keep 11 bits down to 2^-24 of the largest contribution and are off by at most 2^-35 of it below that, which
@@ -535,7 +535,7 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
         float by[NC];                      // what sums and accumulators are multiplied by
 #pragma unroll
         for (int c = 0; c < NC; ++c) by[c] = 1.f;
-        const float floor = unit * 0x1p-60f, page_scale = !ValueCodes<D, WIDE, L>::kRaw || held ? v.scale : 0.f, scale = fmaxf(page_scale, floor), add = __builtin_amdgcn_logf(scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(scale);
+        const float floor = unit * 0x1p-60f, page_scale = !ValueCodes<D, WIDE, L>::kRaw || held ? v.scale : 0.f, scale = fmaxf(fabsf(page_scale), floor), add = __builtin_amdgcn_logf(scale) - log_unit, back = unit * __builtin_amdgcn_rcpf(scale);
         const bool tiny = __any(!(page_scale >= floor)), early = masked || fresh;
         bool moved = early;
 #pragma unroll
@@ -548,7 +548,7 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
                 moved = true;
                 w[c] = exponentials(s[c], f, add - m[c], sum);
             }
-            if (__builtin_expect(tiny, 0)) w[c] = exponentials(s[c], f, add - m[c], sum, page_scale >= floor ? 1.f : page_scale / floor);
+            if (__builtin_expect(tiny, 0)) w[c] = exponentials(s[c], f, add - m[c], sum, page_scale >= floor ? 1.f : page_scale / scale);
             l[c] = fmaf(sum, back, l[c] * by[c]);
         }
         if (__builtin_expect(fresh, 0)) {

@@ -966,3 +966,42 @@ def test_rotary_has_a_tangent(dev):
             assert all(torch.equal(a, b) for a, b in zip([g.primal for g in got] + [g.tangent for g in got], want))
         dq = ad.unpack_dual(torch.autograd.grad(y[0], leaf, ad.make_dual(w, tq))[0])
         assert torch.equal(dq.primal, ops.rotary_axes_bwd(w, None, *how)[0]) and torch.equal(dq.tangent, ops.rotary_axes_bwd(tq, None, *how)[0])
+
+
+@pytest.mark.parametrize("new", [1, 5, 80])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_negative_scales(dev, new, dim):
+    """A stored value is code times scale, whatever the scale's sign; the first page's is negative too."""
+    rng, gen = random.Random(new), torch.Generator().manual_seed(new)
+    page, heads, kv_heads, lens = 16, 8, 2, [new + 333, new + 40]
+    kc, ks = random_cache(gen, 60, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, 60, kv_heads, page, dim, E4M3, dev)
+    table = make_table(rng, lens, page, -(-max(lens) // page), 60)
+    ks *= torch.where(torch.rand(60, kv_heads, generator=gen) < 0.5, -1.0, 1.0).to(dev)
+    vs *= torch.where(torch.rand(60, kv_heads, generator=gen) < 0.5, -1.0, 1.0).to(dev)
+    vs[int(table[0, 0])] = -2.0 ** -5
+    q = torch.randn(2 * new, heads, dim, generator=gen).to(BF)
+    for t in (table, widen(table, page)):
+        check_attention(dev, q, (kc, vc, ks, vs), t, lens, [0, new, 2 * new], dim ** -0.5, max_query_len=new)
+    vs.fill_(-0.25)
+    check_attention(dev, q, (kc, vc, ks, vs), table, lens, [0, new, 2 * new], dim ** -0.5, max_query_len=new)
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+def test_append_behind_a_negative_scale(dev, code):
+    """A page written elsewhere with a negative scale: its scale turns positive, its values stay (to one rounding)."""
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(1)
+    kc, _ = random_cache(gen, 3, 1, 16, 64, code, dev)
+    vc, _ = random_cache(gen, 3, 1, 16, 64, code, dev)
+    ks, vs = (torch.tensor([[-2.0 ** -5], [-1.0], [-2.0 ** -9]], device=dev) for _ in range(2))
+    before = [codes_of(c) * s.cpu().double()[..., None, None] for c, s in ((kc, ks), (vc, vs))]
+    x = torch.randn(3, 1, 64, generator=gen).to(BF)
+    x[0, 0, 0] = 100.0
+    ops.paged_kv_append(x.to(dev), x.to(dev), kc, vc, ks, vs, torch.tensor([7, 16 + 7, 32 + 7], device=dev))
+    for c, s, had in ((kc, ks, before[0]), (vc, vs, before[1])):
+        assert bool((s > 0).all())
+        now = codes_of(c) * s.cpu().double()[..., None, None]
+        step = s.cpu().double()[..., None, None] * (0.5 if code == INT8 else 2.0 ** -10)
+        assert bool(((now - had)[:, :, :7].abs() <= (step if code == INT8 else torch.maximum(step, had[:, :, :7].abs() * 2.0 ** -4))).all())
+        assert bool(((now[:, :, 7] - x.double()).abs() <= torch.maximum(s.cpu().double()[..., None] * (0.5 if code == INT8 else 2.0 ** -10), x.double().abs() * (0 if code == INT8 else 2.0 ** -4))).all())
