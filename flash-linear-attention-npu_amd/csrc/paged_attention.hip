@@ -28,11 +28,11 @@ int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *
                     FLA_ERR_SHAPE, "%s: rows of %s must be contiguous and 16-byte aligned.", op, t == q ? "query" : "out");
     }
     FLA_REQUIRE(separate(out), FLA_ERR_SHAPE, "%s: rows of out overlap.", op);
-    if ((rc = check_tensor(table, op, "block_table", 2, dt_bit(FLA_I32)))) return rc;
+    if ((rc = check_table(op, table))) return rc;
     if ((rc = check_tensor(lens, op, "seq_lens", 1, dt_bit(FLA_I32)))) return rc;
     const int64_t n = table->shape[0];
     FLA_REQUIRE(lens->shape[0] == n && is_contiguous(lens), FLA_ERR_SHAPE, "%s: seq_lens must be a contiguous tensor of %lld elements.", op, (long long)n);
-    FLA_REQUIRE(inner_unit(table) && table->stride[0] >= 0, FLA_ERR_SHAPE, "%s: block_table must have unit innermost stride.", op);
+    FLA_REQUIRE(table->shape[1] == 0 || (inner_unit(table) && table->stride[0] >= 0), FLA_ERR_SHAPE, "%s: block_table must have unit innermost stride.", op);
     if (present(cu)) {
         if ((rc = check_tensor(cu, op, "cu_seqlens", 1, dt_bit(FLA_I32)))) return rc;
         FLA_REQUIRE(cu->shape[0] == n + 1 && is_contiguous(cu), FLA_ERR_SHAPE, "%s: cu_seqlens must be a contiguous tensor of %lld elements.", op, (long long)(n + 1));

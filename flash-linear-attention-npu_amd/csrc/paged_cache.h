@@ -11,6 +11,12 @@ struct CacheShape {
     int shift = 0, code = 0;
 };
 
+// The pages of each request, i32 [N,M]; a table without columns has no data.
+inline int check_table(const char *op, const fla_tensor *table) {
+    const bool empty = table != nullptr && table->ndim == 2 && table->dtype == FLA_I32 && table->shape[0] >= 0 && table->shape[1] == 0;
+    return empty ? FLA_OK : check_tensor(table, op, "block_table", 2, dt_bit(FLA_I32));
+}
+
 // `like`: the shape the cache must have (the value cache against the key cache), or NULL
 inline int check_cache(const char *op, const char *name, const fla_tensor *cache, const char *scales_name, const fla_tensor *scales,
                        const CacheShape *like, CacheShape &shape) {

@@ -9,6 +9,7 @@
 // tokens in pages of 16 6.4 us (a launch alone: 1.8 us); four tokens a thread: 9.7 us.
 #include "common.h"
 #include "device_utils.h"
+#include "paged_cache.h"
 
 namespace fla {
 namespace {
@@ -163,9 +164,9 @@ int plan_impl(const fla_tensor *context, const fla_tensor *query, const fla_tens
               hipStream_t stream) {
     const char *op = "paged_kv_plan";
     int rc;
-    if ((rc = check_tensor(table, op, "block_table", 2, dt_bit(FLA_I32)))) return rc;
+    if ((rc = check_table(op, table))) return rc;
     const int64_t n = table->shape[0], width = table->shape[1];
-    FLA_REQUIRE(inner_unit(table) && table->stride[0] >= 0 && (n <= 1 || table->stride[0] >= width), FLA_ERR_SHAPE,
+    FLA_REQUIRE(width == 0 || (inner_unit(table) && table->stride[0] >= 0 && (n <= 1 || table->stride[0] >= width)), FLA_ERR_SHAPE,
                 "%s: block_table must have unit innermost stride and rows that do not overlap.", op);
     FLA_REQUIRE(block_size >= 16 && block_size <= 256 && (block_size & (block_size - 1)) == 0, FLA_ERR_UNSUPPORTED,
                 "%s: block_size must be a power of two from 16 to 256, got %lld.", op, (long long)block_size);

@@ -472,3 +472,10 @@ def test_rotary_refuses_results_that_two_rows_share(lib):
     for out in (dict(q_out=desc((5, 2, 16), BF16, (16, 16, 1))), dict(k_out=desc((5, 1, 16), BF16, (8, 16, 1)))):
         args, keep = rotary_args(**out)
         assert fn(*args, None) == SHAPE and "rows of an output overlap" in lib.fla_last_error().decode()
+
+
+def test_a_table_without_columns_needs_no_memory(lib):
+    status, size, text = query(lib, attention_args(block_table=desc((3, 0), I32, data=0)))
+    assert (status, size) == (OK, 0), text
+    assert query(lib, attention_args(block_table=desc((3, 0), I64, data=0)))[0] == NULL
+    assert query(lib, attention_args(block_table=desc((3, 4), I32, data=0)))[0] == NULL

@@ -1005,3 +1005,18 @@ def test_append_behind_a_negative_scale(dev, code):
         step = s.cpu().double()[..., None, None] * (0.5 if code == INT8 else 2.0 ** -10)
         assert bool(((now - had)[:, :, :7].abs() <= (step if code == INT8 else torch.maximum(step, had[:, :, :7].abs() * 2.0 ** -4))).all())
         assert bool(((now[:, :, 7] - x.double()).abs() <= torch.maximum(s.cpu().double()[..., None] * (0.5 if code == INT8 else 2.0 ** -10), x.double().abs() * (0 if code == INT8 else 2.0 ** -4))).all())
+
+
+def test_tables_without_columns(dev):
+    """Requests that cannot hold a page: no token has a slot, no row sees anything."""
+    from fla_hip import ops
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    gen = torch.Generator().manual_seed(0)
+    table = torch.empty(2, 0, dtype=torch.int32, device=dev)
+    slots, pos, cu, seq, used, _ = ops.paged_kv_plan(i32([0, 4]), i32([2, 1]), table, i32([5]), 16, 4)
+    assert slots.tolist() == [-1] * 4 and pos.tolist() == [0, 1, 4, 0] and cu.tolist() == [0, 2, 3] and seq.tolist() == [2, 5] and used.tolist() == [0]
+    kc, ks = random_cache(gen, 4, 1, 16, 64, E4M3, dev)
+    for rows in (2, 300):
+        q = torch.randn(rows, 4, 64, device=dev).to(BF)
+        out, lse = ops.paged_kv_attention(q, kc, kc, ks, ks, table, i32([3, 500]), i32([0, 1, rows]), return_lse=True)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
