@@ -265,7 +265,8 @@ int append_impl(const fla_tensor *key, const fla_tensor *value, const fla_tensor
     int rc;
     CacheShape shape;
     AppendParams p{};
-    const fla_tensor *x[2] = {key, value}, *cache[2] = {key_cache, value_cache}, *scales[2] = {key_scales, value_scales};
+    const Folded rows[2] = {Folded(key), Folded(value)}, codes[2] = {Folded(key_cache), Folded(value_cache)}, steps[2] = {Folded(key_scales), Folded(value_scales)};
+    const fla_tensor *x[2] = {rows[0], rows[1]}, *cache[2] = {codes[0], codes[1]}, *scales[2] = {steps[0], steps[1]};
     for (int i = 0; i < 2; ++i) {
         if ((rc = check_cache(op, i ? "value_cache" : "key_cache", cache[i], i ? "value_scales" : "key_scales", scales[i], i ? &shape : nullptr, shape))) return rc;
         if ((rc = check_tensor(x[i], op, i ? "value" : "key", 3, i ? dt_bit(key->dtype) : dt_bit(FLA_BF16) | dt_bit(FLA_F16) | dt_bit(FLA_F32)))) return rc;

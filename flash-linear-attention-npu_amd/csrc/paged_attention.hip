@@ -6,12 +6,14 @@ namespace {
 
 inline bool present(const fla_tensor *t) { return t != nullptr && t->data != nullptr; }
 
-int attention_impl(const fla_tensor *q, const fla_tensor *kc, const fla_tensor *vc, const fla_tensor *ks, const fla_tensor *vs,
+int attention_impl(const fla_tensor *q_, const fla_tensor *kc_, const fla_tensor *vc_, const fla_tensor *ks_, const fla_tensor *vs_,
                    const fla_tensor *table, const fla_tensor *lens, const fla_tensor *cu, double scale, int64_t max_query_len,
-                   bool clear_tail, const fla_tensor *out, const fla_tensor *lse, void *workspace, uint64_t size, hipStream_t stream,
+                   bool clear_tail, const fla_tensor *out_, const fla_tensor *lse_, void *workspace, uint64_t size, hipStream_t stream,
                    uint64_t *query) {
     const char *op = "paged_kv_attention";
     int rc;
+    const Folded fq(q_), fkc(kc_), fvc(vc_), fks(ks_), fvs(vs_), fout(out_), flse(lse_);
+    const fla_tensor *q = fq, *kc = fkc, *vc = fvc, *ks = fks, *vs = fvs, *out = fout, *lse = flse;
     CacheShape shape;
     if ((rc = check_cache(op, "key_cache", kc, "key_scales", ks, nullptr, shape))) return rc;
     if ((rc = check_cache(op, "value_cache", vc, "value_scales", vs, &shape, shape))) return rc;

@@ -11,6 +11,17 @@ struct CacheShape {
     int shift = 0, code = 0;
 };
 
+// A descriptor whose extents of one have stride 0: theirs leads nowhere and may be anything.
+struct Folded {
+    fla_tensor t;
+    const fla_tensor *from;
+    explicit Folded(const fla_tensor *x) : t(x ? *x : fla_tensor{}), from(x) {
+        for (int i = 0; i < t.ndim && i < FLA_MAX_DIMS; ++i)
+            if (t.shape[i] == 1) t.stride[i] = 0;
+    }
+    operator const fla_tensor *() const { return from ? &t : nullptr; }
+};
+
 // The pages of each request, i32 [N,M]; a table without columns has no data.
 inline int check_table(const char *op, const fla_tensor *table) {
     const bool empty = table != nullptr && table->ndim == 2 && table->dtype == FLA_I32 && table->shape[0] >= 0 && table->shape[1] == 0;

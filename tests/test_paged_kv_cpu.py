@@ -479,3 +479,16 @@ def test_a_table_without_columns_needs_no_memory(lib):
     assert (status, size) == (OK, 0), text
     assert query(lib, attention_args(block_table=desc((3, 0), I64, data=0)))[0] == NULL
     assert query(lib, attention_args(block_table=desc((3, 4), I32, data=0)))[0] == NULL
+
+
+def test_strides_of_extents_of_one_may_be_anything(lib):
+    one = dict(query=desc((1, 8, 128), BF16, (3, 128, 1)), out=desc((1, 8, 128), BF16, (1, 128, 1)), lse=desc((1, 8), F32, (0, 1)),
+               key_cache=desc((1, 2, 16, 128), F8, (5, 2048, 128, 1)), value_cache=desc((1, 2, 16, 128), F8, (0, 2048, 128, 1)),
+               key_scales=desc((1, 2), F32, (0, 1)), value_scales=desc((1, 2), F32, (1, 1)))
+    status, _, text = query(lib, attention_args(**one))
+    assert status == OK, text
+    single = dict(query=desc((6, 4, 64), BF16), out=desc((6, 4, 64), BF16), lse=None, key_cache=desc((10, 1, 16, 64), F8, (1024, 1, 64, 1)),
+                  value_cache=desc((10, 1, 16, 64), F8, (1024, 1 << 40, 64, 1)), key_scales=desc((10, 1), F32), value_scales=desc((10, 1), F32))
+    status, _, text = query(lib, attention_args(**single))
+    assert status == OK, text
+    assert query(lib, attention_args(query=desc((1, 8, 128), BF16, (3, 64, 1)), out=desc((1, 8, 128), BF16, (3, 64, 1))))[0] == SHAPE

@@ -1020,3 +1020,33 @@ def test_tables_without_columns(dev):
         q = torch.randn(rows, 4, 64, device=dev).to(BF)
         out, lse = ops.paged_kv_attention(q, kc, kc, ks, ks, table, i32([3, 500]), i32([0, 1, rows]), return_lse=True)
         assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_strides_of_extents_of_one(dev):
+    """One token taken out of a long buffer, one head, one page: the stride of an extent of one leads nowhere and may be anything."""
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(0)
+    page, heads, dim = 16, 4, 64
+    one = lambda x, at: x.as_strided(x.shape, at)
+    long = torch.randn(1, (1 << 21) // (heads * dim) + 5, heads, dim, generator=gen).to(BF).to(dev)
+    kv = long[:, 7]                                           # [1, heads, dim], 2^21 elements to the next batch entry
+    assert kv.stride(0) >= 1 << 21
+    kc, ks = random_cache(gen, 1, heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, 1, heads, page, dim, E4M3, dev)
+    q = torch.randn(1, heads * 2, dim, generator=gen).to(BF).to(dev)
+    slots, table, lens = torch.tensor([3], device=dev), torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.tensor([4], dtype=torch.int32, device=dev)
+    plain = [clone_strided(kc), clone_strided(vc), ks.clone(), vs.clone()]
+    ops.paged_kv_append(kv.contiguous(), kv.contiguous(), *plain, slots)
+    want = ops.paged_kv_attention(q, *plain, table, lens)
+    odd = [one(c, (7, page * dim, dim, 1)) for c in (kc, vc)]
+    odd += [one(s, (0, 1)) for s in (ks, vs)]
+    ops.paged_kv_append(kv, kv, *odd, slots)
+    got = ops.paged_kv_attention(one(q, (3, dim, 1)), *odd, table, lens, out=one(torch.empty_like(q), (5, dim, 1)))
+    assert torch.equal(got, want) and torch.equal(codes_of(kc), codes_of(plain[0])) and torch.equal(ks, plain[2])
+    flat = torch.randn(page, dim, generator=gen)
+    single = torch.zeros(6, 1, page, dim, dtype=torch.uint8, device=dev).view(E4M3)
+    s1 = torch.ones(6, 1, device=dev)
+    single.view(torch.uint8).copy_(flat.to(E4M3).view(torch.uint8).to(dev))
+    a = ops.paged_kv_attention(q, single, single, s1, s1, table + 2, lens)
+    b = ops.paged_kv_attention(q, one(single, (page * dim, 1, dim, 1)), one(single, (page * dim, 3, dim, 1)), s1, s1, table + 2, lens)
+    assert torch.equal(a, b)
