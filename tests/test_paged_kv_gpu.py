@@ -1050,3 +1050,57 @@ def test_strides_of_extents_of_one(dev):
     a = ops.paged_kv_attention(q, single, single, s1, s1, table + 2, lens)
     b = ops.paged_kv_attention(q, one(single, (page * dim, 1, dim, 1)), one(single, (page * dim, 3, dim, 1)), s1, s1, table + 2, lens)
     assert torch.equal(a, b)
+
+
+def test_rotary_gradient_replays_from_a_graph(dev):
+    """Forward and gradient captured together; inputs, positions and gradients change between replays, eager calls run in between."""
+    from fla_hip import ops
+    gen = torch.Generator().manual_seed(6)
+    rn = lambda *s: torch.randn(*s, generator=gen).to(BF)
+    q, k = rn(40, 4, 64).to(dev).requires_grad_(), rn(40, 2, 64).to(dev).requires_grad_()
+    dq, dk, pos = rn(40, 4, 64).to(dev), rn(40, 2, 64).to(dev), torch.arange(40, device=dev)[None].contiguous()
+    freq = torch.rand(32, generator=gen).to(dev)
+
+    def both(a, b):
+        y = ops.rotary_axes(a, b, pos, freq, (32,))
+        return [t.detach() for t in y] + list(torch.autograd.grad(y, (a, b), (dq, dk)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(q, k)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = both(q, k)
+    for _ in range(4):
+        with torch.no_grad():
+            for t in (q, k, dq, dk):
+                t.copy_(rn(*t.shape))
+            pos.copy_(torch.randint(0, 1 << 20, pos.shape, generator=gen))
+        eager = both(q.detach().clone().requires_grad_(), k.detach().clone().requires_grad_())
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(static, eager))
+
+
+def test_split_attention_on_two_streams_at_once(dev):
+    """Calls that are joined through workspaces run side by side; each has its own."""
+    from fla_hip import ops
+    rng, gen = random.Random(2), torch.Generator().manual_seed(2)
+    page, heads, kv_heads, dim, lens = 64, 8, 2, 128, [4000, 2500, 70]
+    kc, ks = random_cache(gen, 120, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, 120, kv_heads, page, dim, E4M3, dev)
+    table, seq = make_table(rng, lens, page, 80, 120).to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+    qs = [torch.randn(3, heads, dim, generator=gen).to(BF).to(dev) for _ in range(2)]
+    want = [ops.paged_kv_attention(q, kc, vc, ks, vs, table, seq, return_lse=True) for q in qs]
+    streams, got = [torch.cuda.Stream() for _ in qs], []
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for q, s in zip(qs, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.paged_kv_attention(q, kc, vc, ks, vs, table, seq, return_lse=True))
+    torch.cuda.synchronize()
+    for i, (out, lse) in enumerate(got):
+        assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
