@@ -57,7 +57,8 @@ int attention_impl(const fla_tensor *q_, const fla_tensor *kc_, const fla_tensor
     const int64_t longest = !present(cu) ? 1 : max_query_len ? (max_query_len < T ? max_query_len : T) : T;
     plan.longest_rows = (int)(longest * group < 4096 ? longest * group : 4096);
     // Up to 64 rows of a request go to the decode kernel, in tiles of 16 or 32: it splits the keys among the waves of a
-    // workgroup (48 requests of 1 to 7 rows times 6 heads, contexts to 5 k: tiles of 32 rows 42 us, one of 64 rows 66 us).
+    // workgroup (48 requests of 1 to 7 rows times 6 heads, contexts to 5 k, when measured: tiles of 32 rows 42 us, one of 64
+    // rows 66 us; since then 29 us in tiles of 32).
     const int64_t rows_most = longest * group;
     const bool prefill = rows_most > 64;
     plan.nc = !prefill ? (rows_most <= 16 ? 1 : 2) : dim == 256 ? 2 : 4;
@@ -73,7 +74,10 @@ int attention_impl(const fla_tensor *q_, const fla_tensor *kc_, const fla_tensor
     //    and 211 us);
     //  - tables of at most 2048 tokens: one chunk and one launch, of eight waves (four requests of 1100: 11.6 us against 10.2
     //    to 12.3 us with two launches on the GPU, and one launch less on the host);
-    //  - prefill: only where tiles, of one wave each, would leave compute units idle.
+    //  - prefill: only where tiles, of one wave each, would leave compute units idle: below 2048 (rows behind 4096 tokens, 32
+    //    heads on 8 of 128: 1024 rows split 125 us, whole 247; 2048 rows split 238, whole 297; 4096 rows split 458, whole 431);
+    //  - chunks of at least 256 tokens (one prompt of 256 rows behind 1024: 128 tokens 43 us, 256 40, 512 47; one decode of 2100
+    //    tokens 12.0, 12.1, 13.9; 64 rows behind 1024 would take 40 us with 128 and 44 with 256).
     const int64_t capacity = table->shape[1] << shape.shift, tiles_all = plan.tiles * shape.heads;
     plan.waves = 4;
     p.min_units = 4;

@@ -3,9 +3,10 @@
 // Bound by HBM: each code is read once, with loads that leave the caches alone (a code is not read again in this call).  The
 // waves of a workgroup take 32-token steps of a chunk in turn, each with its own running maximum, sum and accumulators (the
 // walk of paged_attention.h: no LDS, no barrier), and are joined once at the end.
-// Measured, 32 heads on 8 of 128: 128 ragged requests to 8192 tokens 187 us + 5.6 us of join for 1.04 GB; one of 262 k tokens
-// 89 + 5.4 us for 537 MB; four to 1100 tokens 12.0 us (32 workgroups, five steps of 1.2 us: the vector instructions of
-// eight waves); 24 heads on 4 of 64, 48 requests of 1 to 7 rows 23 + 6.6 us.
+// Measured, 32 heads on 8 of 128: 128 ragged requests to 8192 tokens 187 us + 5.7 us of join for 1.04 GB, one of 262 k tokens
+// 89 + 5.4 us for 537 MB (both with a part of the codes in the Infinity Cache); four to 1100 tokens 12.0 us (32 workgroups: 56 %
+// of the waves' time is waiting for lengths, table and codes, 18 % for a turn to issue, 27 % issues); 24 heads on 4 of 64, 48
+// requests of 1 to 7 rows 24 + 6.8 us.
 #include "paged_attention.h"
 
 namespace fla {
@@ -191,7 +192,9 @@ template <int CODE> int launch_dim(const AttnParams &p, const AttnLaunch &plan, 
 template <int ROWS> int launch_join(const AttnParams &p, const AttnLaunch &plan, hipStream_t stream) {
     constexpr int kMany = 16;
     const int rows = plan.longest_rows < ROWS ? plan.longest_rows : ROWS;
-    const bool many = p.target >= 16 * plan.tiles;       // chunks of a tile
+    // 16 waves on a row from 16 chunks of a tile on (decode of 1 x 262 k tokens 93 us, 99 with one wave a row; 1 x 32 k 22 and 28;
+    // 4 x 32 k, 16 chunks, 52.4 and 51.9; 16 x 8 k, 4 chunks, 52.9 and 50.4)
+    const bool many = p.target >= 16 * plan.tiles;
     const dim3 grid((unsigned)(plan.tiles * p.heads), (unsigned)(many ? rows : (rows + 3) / 4));
 #define FLA_JOIN(DD)                                                                                                                           \
     do {                                                                                                                                       \

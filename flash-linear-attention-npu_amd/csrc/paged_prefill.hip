@@ -1,10 +1,11 @@
 // paged_kv_attention for many query rows (chunked prefill): a wave takes 64 of them (32 for D = 256) over all their keys.
 // Bound by the vector and matrix units together.  For a 32-token step and D = 128 a wave issues 64 matrix instructions
 // (1024 clocks of the matrix pipe) and about 230 vector ones, 32 of them exponentials; codes are widened once for 64 rows,
-// straight from the loads of the wave, with no LDS (but for the queries, which would take registers) and no barrier: the
-// tiles of a head run on one XCD, whose L2 holds its keys.  32 rows a wave: 1150 us where 64 take 852.
-// Measured: 2 x 4096 tokens behind 4096, 32 heads on 8 of 128, e4m3: 745 to 770 us = 1070 to 1107 TFLOP/s, 76 to 79 % of what a library
-// product of 8192^3 reaches; int8 845 us; D = 64 515 us; D = 256 1793 us.
+// straight from the loads of the wave, with no LDS (but for the queries, which would take registers) and no barrier: with a
+// multiple of 8 cache heads the tiles of a head run on one XCD, whose L2 holds its keys.  32 rows a wave took 1150 us where 64
+// took 852 (before the priorities of paged_attention.h).
+// Measured: 2 x 4096 tokens behind 4096, 32 heads on 8 of 128, e4m3: 784 to 800 us by card in replays and calls back to back, 1030 to
+// 1050 TFLOP/s, 74 to 75 % of what a library product of 8192^3 reaches; int8 886 to 904 us; D = 64 524 to 540 us; D = 256 1771 to 1815 us.
 #include "paged_attention.h"
 
 namespace fla {

@@ -207,6 +207,8 @@ int rotary_impl(const fla_tensor *q, const fla_tensor *k, const fla_tensor *posi
     p.heads = (int)heads;
     p.dim = (int)dim;
     p.pairs = (int)pairs;
+    // Four tokens a workgroup from 4096 on (32 + 8 heads of 128, all channels, bf16: 256 tokens 4.4 us with one and 6.1 with four,
+    // 2048 9.8 and 10.4, 4096 16.7 and 16.0, 8192 34.4 and 34.3; at 32768 one is ahead again, 117 and 125).
     p.tokens_per_wg = tokens >= 4096 ? kMaxTokens : 1;
     const int64_t groups = (tokens + p.tokens_per_wg - 1) / p.tokens_per_wg;
     FLA_REQUIRE(groups * kThreads < ((int64_t)1 << 32), FLA_ERR_SHAPE, "%s: too many tokens.", op);

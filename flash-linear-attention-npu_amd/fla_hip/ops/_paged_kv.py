@@ -218,8 +218,8 @@ def rotary_axes_bwd(dq, dk, positions, inv_freq, sections, *, axis_order: str = 
 
 def paged_kv_append(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping):
     """Quantises ``key`` and ``value`` ``[T, H, D]`` into the pages that ``slot_mapping`` int64 ``[T]`` names (negative: the row
-    is skipped), as ``paged_kv_plan`` lays them out: the rows of one page follow each other with ascending slots (a page
-    named by two separate runs of rows in one call has unspecified contents).  A page's scale is the smallest power of
+    is skipped), as ``paged_kv_plan`` lays them out: the rows of one page are one run, neighbours with slots that ascend by
+    one (a page named by two separate runs of rows in one call, or by the same slot twice, has unspecified contents).  A page's scale is the smallest power of
     two ``s`` with ``max|x| / s <= 448`` (e4m3) or ``127`` (int8) over the tokens of that page and head so far; when it grows,
     the codes already there are converted.  Tokens of a page before the first new one are kept; a page whose offset 0 is
     written starts afresh.  Infinities store the largest code; NaN stores NaN (e4m3) or 0 (int8)."""
@@ -241,7 +241,8 @@ def paged_kv_attention(query, key_cache, value_cache, key_scales, value_scales, 
     ``cu_seqlens`` int32 ``[N + 1]`` the query rows of each request, or None for one row each (decode).  Row j of a
     request's q rows is token ``seq_lens - q + j`` and sees the tokens up to itself, also in a request that goes on behind the
     last row of ``query``; pages that the table gives a number outside the pool are not seen, and a row that sees nothing is 0 with lse -inf.  ``scale`` defaults to ``D ** -0.5``.
-    ``max_query_len``: the largest number of query rows of a request, if the caller knows it; it only chooses the kernel.
+    ``max_query_len``: the largest number of query rows of a request, if the caller knows it.  It only chooses the kernel, but
+    a batch of few rows each is slower without it (128 requests of one row up to 8192 tokens: 210 us with it, 313 without).
     Rows that belong to no request are 0 in a new result and left as they are in a given ``out``.  Returns ``out`` or, with
     ``return_lse``, ``(out, lse)`` with lse fp32 ``[T, Hq]`` (natural logarithm)."""
     import torch
