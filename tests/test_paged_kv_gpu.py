@@ -917,8 +917,8 @@ def test_a_first_token_that_draws_the_weight_and_holds_no_values(dev, rows, head
         want = p @ vd
         err = (dim + 8) * 2.0 ** -24 * ((x.abs() @ kd.abs().t()) * scale).amax(-1)[:, None]
         peak = p.amax(-1)[:, None]
-        # the result's rounding (8 significant bits: 2^-8 of its value), the weights' (2^-12) and the scores'; codes are at most 4
-        bound = want * (torch.finfo(BF).eps / 2 * 1.01 + 2.0 ** -12 * 1.01 + 2 * err) + n * 2.0 ** -35 * peak * 4 + torch.finfo(BF).tiny
+        # the result's rounding (8 significant bits: 2^-8 of its value), the weights' (11: 2^-11) and the scores'; codes are at most 4
+        bound = want * (torch.finfo(BF).eps / 2 * 1.01 + torch.finfo(F16).eps / 2 * 1.01 + 2 * err) + n * 2.0 ** -35 * peak * 4 + torch.finfo(BF).tiny
         error = (out[:, h].double() - want).abs()
         assert bool((error <= bound).all()), (h, float((error / bound).max()), float((error / want).max()))
         want_lse = score.logsumexp(-1)
