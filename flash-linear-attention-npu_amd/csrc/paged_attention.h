@@ -280,6 +280,12 @@ __device__ __forceinline__ float scale_unit(const AttnParams &p, const int32_t *
     return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, fminf(fmaxf(s, 0x1p-60f), 0x1p60f)) & 0x7f800000u);
 }
 
+// Natural logarithm of 2^m l.  The exponent of l joins m first: beside pages with a scale of 0 both are far from 0 (m counts their
+// value scale as 2^-60 u, l takes it out again), and a logarithm of l rounded there would cost what their sum keeps.
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return ((m + (float)__builtin_amdgcn_frexp_expf(l)) + log2f(__builtin_amdgcn_frexp_mantf(l))) * (1.f / kLog2e);
+}
+
 // One wave: 16 NC query rows against the tokens it is led over, 32 at a time.
 //   S^T = K Q^T: tokens are the rows of the accumulators, query rows their columns; O^T += V^T P^T with P^T straight from
 //   the accumulator layout.
@@ -659,7 +665,7 @@ template <int CODE, int D, int NC, bool WIDE, Loads L> struct Walk {
                         }
                     }
                 }
-                if (p.lse && g == 0) p.lse[(int64_t)(rq.first + tok) * p.lse_t + (int64_t)h * p.lse_h] = (mm[c] + log2f(ll[c])) * (1.f / kLog2e);
+                if (p.lse && g == 0) p.lse[(int64_t)(rq.first + tok) * p.lse_t + (int64_t)h * p.lse_h] = log_sum(mm[c], ll[c]);
             } else {
                 const int64_t slot = (item * p.heads + head) * rows_per_tile + in_tile;
 #pragma unroll

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(64 * (WAVES > 4 ? WAVES : 4)) paged_join_kerne
             elem *dst = static_cast<elem *>(p.out) + (int64_t)(rq.first + tok) * p.o_t + (int64_t)h * p.o_h;
 #pragma unroll
             for (int x = 0; x < V; ++x) dst[lane * V + x] = (elem)(sum.o[x] * by);
-            if (p.lse && lane == 0) p.lse[(int64_t)(rq.first + tok) * p.lse_t + (int64_t)h * p.lse_h] = (sum.m + log2f(sum.l)) * (1.f / kLog2e);
+            if (p.lse && lane == 0) p.lse[(int64_t)(rq.first + tok) * p.lse_t + (int64_t)h * p.lse_h] = log_sum(sum.m, sum.l);
         }
         if (WAVES > 1) __syncthreads();
     }

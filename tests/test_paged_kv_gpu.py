@@ -1104,3 +1104,27 @@ def test_split_attention_on_two_streams_at_once(dev):
     torch.cuda.synchronize()
     for i, (out, lse) in enumerate(got):
         assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
+
+
+@pytest.mark.parametrize("new", [1, 3, 80])
+def test_log_sums_beside_pages_with_a_scale_of_zero(dev, new):
+    """Values of 0 do not enter the sum of the softmax.  Many small texts.  Bound: the scores' error, (D + 8) * 2^-24 of sum |q||k| * scale,
+    and 2^-21 of 1 + |lse| (exponents up to 16 are rounded by 2^-21, times ln 2; the sums and the logarithm by less)."""
+    from fla_hip import ops
+    rng, gen = random.Random(new), torch.Generator().manual_seed(new)
+    page, heads, kv_heads, dim, n = 16, 12, 3, 64, 60 if new < 80 else 6
+    lens = [new + rng.choice([0, 1, 2, 9, 40]) for _ in range(n)]
+    pool = sum(-(-m // page) for m in lens) + 2
+    kc, ks = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    vc, vs = random_cache(gen, pool, kv_heads, page, dim, E4M3, dev)
+    table = make_table(rng, lens, page, -(-max(lens) // page), pool)
+    q = torch.randn(n * new, heads, dim, generator=gen).to(F16)
+    cu = [new * r for r in range(n + 1)]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    _, want, _, reach, _ = ref.attention(q, codes_of(kc), codes_of(vc), ks.cpu(), vs.cpu(), table, lens, cu, -0.1)
+    for zero in (slice(0, None, 2), slice(None)):
+        vs[zero] = 0
+        for t in (table, widen(table, page)):
+            _, lse = ops.paged_kv_attention(q.to(dev), kc, vc, ks, vs, t.to(dev), i32(lens), i32(cu), scale=-0.1, max_query_len=new, return_lse=True)
+            error, bound = (lse.cpu().double() - want).abs(), (dim + 8) * 2.0 ** -24 * reach + 2.0 ** -21 * (1 + want.abs())
+            assert bool((error <= bound).all()), (float((error / bound).max()), float(error.max()))
