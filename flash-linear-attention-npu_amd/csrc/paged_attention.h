@@ -300,6 +300,7 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 //    pages are.  The sum of the softmax is that of w u / vs.  u, the scale of the request's first page as a power of two,
 //    only keeps these numbers inside fp32.  A scale below 2^-60 u (0 above all) counts as 2^-60 u in the exponent and
 //    multiplies the weight by the rest; of a negative one the magnitude is in the exponent.
+//    (Where nearly all weight lies on such pages, the others' share is off by at most 2^-95 u of a code for each token.)
 //  - weights are rounded to fp16 with 11 bits: a bf16 weight would add an error as large as the rounding of the result.  (bf16
 //    results are as far from exact as with fp32 weights, 1.7e-3; fp16 ones 2.6e-4 where their own rounding leaves 2.1e-4.)  The
 //    largest contribution stands at 2^10 or more, near the top of fp16, because the sum of the softmax counts light weights in
