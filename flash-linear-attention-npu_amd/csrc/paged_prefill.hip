@@ -4,8 +4,8 @@
 // straight from the loads of the wave, with no LDS (but for the queries, which would take registers) and no barrier: with a
 // multiple of 8 cache heads the tiles of a head run on one XCD, whose L2 holds its keys.  32 rows a wave took 1150 us where 64
 // took 852 (before the priorities of paged_attention.h).
-// Measured: 2 x 4096 tokens behind 4096, 32 heads on 8 of 128, e4m3: 784 to 800 us by card in replays and calls back to back, 1030 to
-// 1050 TFLOP/s, 74 to 75 % of what a library product of 8192^3 reaches; int8 886 to 904 us; D = 64 524 to 540 us; D = 256 1771 to 1815 us.
+// Measured: 2 x 4096 tokens behind 4096, 32 heads on 8 of 128, e4m3: 784 to 807 us by card in replays and calls back to back, 1020 to
+// 1050 TFLOP/s, 73 to 75 % of what a library product of 8192^3 reaches; int8 886 to 904 us; D = 64 524 to 540 us; D = 256 1771 to 1815 us.
 #include "paged_attention.h"
 
 namespace fla {
